@@ -359,6 +359,77 @@ LEWM_API lewm_status lewm_encoder_sync_status(lewm_encoder* enc, void* stream);
 LEWM_API const char* lewm_encoder_last_error(const lewm_encoder* enc);
 LEWM_API void lewm_encoder_destroy(lewm_encoder* enc);
 
+/* ------------------------------------------------------------------ training operators
+ * What a training step of the world model needs beside its matrix products: LayerNorm and the
+ * AdaLN-modulated LayerNorm with their backward passes, and the global gradient norm with
+ * clipping. No context: each call works on the given device and stream, allocates nothing,
+ * keeps nothing and never synchronizes, so it may be captured into a CUDA graph. Two calls
+ * that overlap on the GPU need different workspaces. Results are the same bits on every run
+ * of a shape (no atomics). Errors: text from lewm_last_error(NULL). */
+#define LEWM_TYPE_F32 0
+#define LEWM_TYPE_BF16 1
+#define LEWM_TYPE_F16 2
+
+/* Rows of a norm. group == 0, layer norm (nn.LayerNorm over the last dim, reference
+ * lewm/module.py:44,79,147): a = weight, b = bias, each (width) contiguous or NULL.
+ * group >= 1, adaptive layer norm (modulate(norm(x), shift, scale), reference
+ * lewm/module.py:6-8,96-110): a = scale, b = shift, a row of each for every `group`
+ * consecutive rows of x (rows is a multiple of group). */
+typedef struct lewm_norm_desc {
+  int64_t rows;     /* >= 0 */
+  int64_t width;    /* 1 .. 2^24 */
+  int64_t x_stride; /* elements between rows of x (0: the same row) */
+  int64_t group;
+  int64_t a_stride; /* elements between rows of scale; group >= 1 */
+  int64_t b_stride; /* elements between rows of shift; group >= 1 */
+  int32_t x_type;   /* LEWM_TYPE_* of x, y, dy and dx */
+  int32_t p_type;   /* LEWM_TYPE_* of a, b, da and db */
+  float eps;        /* >= 0 */
+} lewm_norm_desc;
+
+/* y = z a + b (layer norm) or z (1 + a) + b (adaptive), z = (x - mean) / sqrt(var + eps) with
+ * the biased variance of the row; y [rows][width] contiguous. stats (float32 [2][rows]: mean,
+ * then 1 / sqrt(var + eps)) is what the backward pass needs, or NULL. float32 arithmetic, one
+ * rounding at the store. */
+LEWM_API lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void* x, const void* a, const void* b,
+                                       void* y, float* stats, int32_t device, void* stream);
+
+/* Bytes of workspace lewm_norm_backward wants for `desc` (0: none). */
+LEWM_API size_t lewm_norm_workspace(const lewm_norm_desc* desc);
+
+/* Gradients of lewm_norm_forward for the output gradient dy (rows dy_stride elements apart):
+ * dx [rows][width], da and db [width] (layer norm) or [rows / group][width] (adaptive), all
+ * contiguous; any may be NULL. `workspace` holds partial sums during the call (16-byte aligned,
+ * lewm_norm_workspace bytes; unused when da and db are NULL). With no rows the gradients of a
+ * layer norm's weight and bias are the caller's zeros: asking for them is LEWM_INVALID_ARG. */
+LEWM_API lewm_status lewm_norm_backward(const lewm_norm_desc* desc, const void* dy, int64_t dy_stride, const void* x,
+                                        const void* a, const float* stats, void* dx, void* da, void* db,
+                                        void* workspace, size_t workspace_bytes, int32_t device, void* stream);
+
+/* Kinds of gradient norm. */
+#define LEWM_NORM_L2 0  /* sqrt of the sum of squares, accumulated in float64 */
+#define LEWM_NORM_MAX 1 /* largest magnitude */
+
+/* Bytes of workspace of lewm_grad_norm and lewm_grad_clip. */
+#define LEWM_GRAD_WORKSPACE 32768
+
+/* norm_out[0] (device float32) = the norm of all elements of n tensors (n >= 0) taken as one
+ * vector; NaN and infinity propagate. src, counts, types: HOST arrays of n device pointers
+ * (contiguous elements, aligned to the element), element counts >= 0 and LEWM_TYPE_*. The
+ * tables are read before the call returns. */
+LEWM_API lewm_status lewm_grad_norm(const void* const* src, const int64_t* counts, const int32_t* types, int32_t n,
+                                    int32_t kind, void* workspace, float* norm_out, int32_t device, void* stream);
+
+/* dst_i = src_i * min(1, max_norm / (norm + 1e-6)), the global-norm clip of
+ * torch.nn.utils.clip_grad_norm_; a NaN norm makes every element NaN. dst_i == src_i clips in
+ * place (and then writes nothing where the factor is 1); otherwise no dst may overlap any other
+ * tensor of the call. norm_in (device float32): a norm computed before, or NULL to compute it
+ * here. norm_out[0] gets the norm. */
+LEWM_API lewm_status lewm_grad_clip(const void* const* src, void* const* dst, const int64_t* counts,
+                                    const int32_t* types, int32_t n, int32_t kind, float max_norm,
+                                    const float* norm_in, void* workspace, float* norm_out, int32_t device,
+                                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,12 @@ class EncoderDescC(C.Structure):
                 ("proj_norm", C.c_int32), ("proj_eps", C.c_float)]
 
 
+class NormDescC(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("width", C.c_int64), ("x_stride", C.c_int64), ("group", C.c_int64),
+                ("a_stride", C.c_int64), ("b_stride", C.c_int64), ("x_type", C.c_int32), ("p_type", C.c_int32),
+                ("eps", C.c_float)]
+
+
 class PlanTraceC(C.Structure):
     _fields_ = [("costs", C.c_void_p), ("topk_idx", C.c_void_p), ("topk_val", C.c_void_p),
                 ("mean", C.c_void_p), ("std", C.c_void_p), ("candidates", C.c_void_p)]
@@ -110,7 +116,18 @@ SIGNATURES = {
     "lewm_encoder_sync_status": (C.c_int, [C.c_void_p, C.c_void_p]),
     "lewm_encoder_last_error": (C.c_char_p, [C.c_void_p]),
     "lewm_encoder_destroy": (None, [C.c_void_p]),
+    "lewm_norm_forward": (C.c_int, [C.POINTER(NormDescC), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_int32, C.c_void_p]),
+    "lewm_norm_workspace": (C.c_size_t, [C.POINTER(NormDescC)]),
+    "lewm_norm_backward": (C.c_int, [C.POINTER(NormDescC), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int32,
+                                     C.c_void_p]),
+    "lewm_grad_norm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                 C.c_int32, C.c_void_p]),
+    "lewm_grad_clip": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_float,
+                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
 }
+GRAD_WORKSPACE = 32768  # LEWM_GRAD_WORKSPACE
 KERNEL_CLASSES = ("embed", "adaln", "qkv_attn", "out_proj", "fc1", "fc2", "final", "sample", "refit", "prep0", "ffn",
                   "ln_operand", "tile_call", "fp32_cost")
 

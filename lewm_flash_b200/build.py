@@ -15,7 +15,8 @@ PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "liblewm_b200.so"
-SOURCES = ["api.cu", "rollout_kernels.cu", "tile_call.cu", "fp32_path.cu", "icem_kernels.cu", "noalloc.cu", "encoder.cu"]
+SOURCES = ["api.cu", "rollout_kernels.cu", "tile_call.cu", "fp32_path.cu", "icem_kernels.cu", "noalloc.cu", "encoder.cu",
+           "train_norm.cu", "grad_clip.cu"]
 HEADERS = ["lewm_common.cuh", "lewm_internal.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -38,7 +39,7 @@ def _stale() -> bool:
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return LIB
-    cmd = [nvcc(), *ARCH, "-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC",
+    cmd = [nvcc(), *ARCH, "-O3", "-std=c++17", "--threads", "0", "-lineinfo", "-shared", "-Xcompiler", "-fPIC",
            "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
            "-I", str(REPO / "include"), "-o", str(LIB) + ".tmp"]
     if verbose:

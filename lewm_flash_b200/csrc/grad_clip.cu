@@ -1,0 +1,459 @@
+// Global gradient norm over many tensors, and clipping by it.
+//
+//   norm = sqrt(sum over all tensors and elements of g^2), or max |g|
+//   dst  = src * min(1, max_norm / (norm + 1e-6))
+//
+// Bound: bytes. The norm reads every gradient once; the scaling cannot start before the norm
+// is known, so it reads them again (from L2 while they fit its 126 MB) and writes once.
+//
+// Layout: the tensors travel in the kernel's parameters (pointer, count, type and first chunk
+// of each: up to 32 KB, so no copy to the device and nothing a captured graph could find
+// changed). They are cut into chunks of 16 KB, four 16-byte loads for each of a block's 256
+// threads; persistent blocks take chunks in a fixed stride and look up a chunk's tensor by
+// bisection. Lists longer than a table take several launches that share the partial sums.
+//
+// The sum of squares of a 16-byte vector is float32 (at most 8 products of like sign) and joins
+// a float64 sum per thread; where that float32 sum is too small or too large for its squares
+// to be normal numbers the vector is summed again in float64. Each block
+// leaves one partial; the scaling blocks each add all partials in the same fixed order, which
+// saves a launch and needs no atomics: the same bits on every run.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+#include "lewm_b200.h"
+#include "lewm_common.cuh"
+#include "lewm_internal.h"
+
+namespace lewm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunkBytes = 16384;  // 4 vectors of 16 bytes per thread
+constexpr int kSlots = 2048;        // partial sums of all launches of a call
+constexpr int kBlocks = 148 * 8;    // 148 SMs x 8 blocks of 256 threads
+static_assert(kBlocks <= kSlots && kSlots * sizeof(double) + 16 <= LEWM_GRAD_WORKSPACE, "workspace");
+
+// A launch's tensors. Element types and whether a tensor's vectors can be 16 bytes (src and
+// dst at the same offset from a 16-byte boundary) share a byte.
+template <int N>
+struct Table {
+  const void* src[N];
+  void* dst[N];
+  int64_t count[N];
+  uint32_t first[N + 1];  // chunk number of each tensor's first chunk; [n] = all chunks
+  uint8_t kind[N];        // LEWM_TYPE_* | 4 if only single elements can be moved
+  int n;
+};
+constexpr int kSmall = 64, kLarge = 1024;
+constexpr int kMaxTensors = 1 << 20;  // 1024 launches of the norm, each with a partial sum at least
+static_assert(sizeof(Table<kLarge>) + 64 <= 32764, "kernel parameters");
+
+// ------------------------------------------------------------------ a chunk of a tensor
+__device__ __forceinline__ float elem(float v) { return v; }
+__device__ __forceinline__ float elem(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float elem(__half v) { return __half2float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+
+// Elements of a chunk: a vector body [v0, v1) of 16-byte vectors counted from the tensor's
+// first 16-byte boundary (element `head`), and single elements [0, head) and [tail, count),
+// which belong to the first and the last chunk.
+template <typename T>
+struct Span {
+  static constexpr int E = 16 / sizeof(T);
+  int64_t head, body, v0, v1;  // body: vectors of the whole tensor
+  __device__ __forceinline__ Span(const T* p, int64_t count, uint32_t chunk) {
+    const int64_t off = (reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T);
+    head = min((E - off) % E, count);
+    body = (count - head) / E;
+    v0 = min((int64_t)chunk * (kChunkBytes / 16), body);
+    v1 = min(v0 + kChunkBytes / 16, body);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ int find_tensor(const Table<N>& t, uint32_t chunk) {
+  int lo = 0, hi = t.n;  // first[lo] <= chunk < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.first[mid] <= chunk) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// ------------------------------------------------------------------ norm
+// A thread's accumulator: float64 sum of squares, or the bits of the largest magnitude (as
+// unsigned integers finite < infinity < NaN).
+template <bool MAX>
+struct Acc {
+  double sum = 0.0;
+  uint32_t bits = 0;
+  // K values; squares between 2^-100 and 2^126 summed in float32, others in float64.
+  template <int K>
+  __device__ __forceinline__ void add(const float* f) {
+    if constexpr (MAX) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) bits = max(bits, __float_as_uint(f[k]) & 0x7fffffffu);
+    } else {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) s = fmaf(f[k], f[k], s);
+      if (s >= 0x1p-100f && s <= 0x1p126f) {
+        sum += (double)s;
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < K; ++k) sum = fma((double)f[k], (double)f[k], sum);
+      }
+    }
+  }
+};
+
+template <typename T, bool MAX>
+__device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t chunk, uint32_t chunks, Acc<MAX>& acc) {
+  using S = Span<T>;
+  const S sp(p, count, chunk);
+  const uint4* v = reinterpret_cast<const uint4*>(p + sp.head);
+  uint4 raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
+    raw[i] = k < sp.v1 ? v[k] : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (sp.v0 + i * kThreads + threadIdx.x >= sp.v1) break;
+    const T* e = reinterpret_cast<const T*>(&raw[i]);
+    float f[S::E];
+#pragma unroll
+    for (int j = 0; j < S::E; ++j) f[j] = elem(e[j]);
+    acc.template add<S::E>(f);
+  }
+  if (chunk == 0 && (int64_t)threadIdx.x < sp.head) {
+    const float f = elem(p[threadIdx.x]);
+    acc.template add<1>(&f);
+  }
+  if (chunk == chunks - 1) {
+    const int64_t k = sp.head + sp.body * S::E + threadIdx.x;
+    if (k < count) {
+      const float f = elem(p[k]);
+      acc.template add<1>(&f);
+    }
+  }
+}
+
+// The block's total of `acc` in thread 0 (as a double: the sum, or the magnitude's bits).
+template <bool MAX>
+__device__ __forceinline__ double block_total(const Acc<MAX>& acc) {
+  __shared__ double warp_part[kThreads / 32];
+  double v = MAX ? (double)acc.bits : acc.sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? fmax(v, w) : v + w;
+  }
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = warp_part[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) v = MAX ? fmax(v, warp_part[w]) : v + warp_part[w];
+  __syncthreads();
+  return v;
+}
+
+// Norm of `slots` partials: the same order in every block, so the same bits.
+template <bool MAX>
+__device__ __forceinline__ float join_partials(const double* part, int slots) {
+  Acc<MAX> acc;
+  for (int i = threadIdx.x; i < slots; i += kThreads) {
+    if constexpr (MAX) acc.bits = max(acc.bits, (uint32_t)part[i]);
+    else acc.sum += part[i];
+  }
+  const double v = block_total<MAX>(acc);
+  return MAX ? __uint_as_float((uint32_t)v) : (float)sqrt(v);
+}
+
+template <int N, bool MAX>
+__global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ Table<N> t, double* part) {
+  griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
+  Acc<MAX> acc;
+  const uint32_t all = t.first[t.n];
+  for (uint32_t c = blockIdx.x; c < all; c += gridDim.x) {
+    const int i = find_tensor(t, c);
+    const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
+    switch (t.kind[i] & 3) {
+      case LEWM_TYPE_F32: chunk_norm(static_cast<const float*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
+      case LEWM_TYPE_BF16:
+        chunk_norm(static_cast<const __nv_bfloat16*>(t.src[i]), t.count[i], chunk, chunks, acc);
+        break;
+      default: chunk_norm(static_cast<const __half*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
+    }
+  }
+  const double v = block_total<MAX>(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = v;
+}
+
+template <bool MAX>
+__global__ void __launch_bounds__(kThreads) k_norm_out(const double* part, int slots, float* norm_out) {
+  griddep_wait();
+  const float norm = join_partials<MAX>(part, slots);
+  if (threadIdx.x == 0) *norm_out = norm;
+}
+
+// ------------------------------------------------------------------ scaling
+template <typename T>
+__device__ __forceinline__ void chunk_scale(const T* src, T* dst, int64_t count, uint32_t chunk, uint32_t chunks,
+                                            bool single, float coef) {
+  using S = Span<T>;
+  if (single) {
+    // src and dst lie differently to 16-byte boundaries: element by element, in chunks of as
+    // many elements as vectors would move.
+    const int64_t e0 = (int64_t)chunk * (kChunkBytes / sizeof(T));
+    const int64_t e1 = chunk == chunks - 1 ? count : e0 + kChunkBytes / sizeof(T);
+    for (int64_t k = e0 + threadIdx.x; k < e1; k += kThreads) put(dst + k, elem(src[k]) * coef);
+    return;
+  }
+  const S sp(src, count, chunk);
+  const uint4* v = reinterpret_cast<const uint4*>(src + sp.head);
+  uint4* o = reinterpret_cast<uint4*>(dst + sp.head);
+  uint4 raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
+    if (k < sp.v1) raw[i] = v[k];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
+    if (k >= sp.v1) break;
+    T* e = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+    for (int j = 0; j < S::E; ++j) put(e + j, elem(e[j]) * coef);
+    o[k] = raw[i];
+  }
+  if (chunk == 0 && (int64_t)threadIdx.x < sp.head) put(dst + threadIdx.x, elem(src[threadIdx.x]) * coef);
+  if (chunk == chunks - 1) {
+    const int64_t k = sp.head + sp.body * S::E + threadIdx.x;
+    if (k < count) put(dst + k, elem(src[k]) * coef);
+  }
+}
+
+// Factor of the clip; a NaN norm gives NaN, as min(1, NaN) must not hide it.
+__device__ __forceinline__ float clip_factor(float norm, float max_norm) {
+  const float c = max_norm / (norm + 1e-6f);
+  return c > 1.f ? 1.f : c;
+}
+
+template <int N, bool MAX>
+__global__ void __launch_bounds__(kThreads) k_grad_scale(const __grid_constant__ Table<N> t, const double* part,
+                                                         int slots, const float* norm_in, float max_norm,
+                                                         float* norm_out, int in_place) {
+  griddep_wait();
+  const float norm = norm_in ? *norm_in : join_partials<MAX>(part, slots);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  const float coef = clip_factor(norm, max_norm);
+  if (in_place && coef == 1.f) return;  // every element times 1 is itself
+  const uint32_t all = t.first[t.n];
+  // Last chunks first: they are what the norm left in L2 when the gradients exceed it.
+  for (uint32_t k = blockIdx.x; k < all; k += gridDim.x) {
+    const uint32_t c = all - 1 - k;
+    const int i = find_tensor(t, c);
+    const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
+    const bool single = t.kind[i] & 4;
+    switch (t.kind[i] & 3) {
+      case LEWM_TYPE_F32:
+        chunk_scale(static_cast<const float*>(t.src[i]), static_cast<float*>(t.dst[i]), t.count[i], chunk, chunks,
+                    single, coef);
+        break;
+      case LEWM_TYPE_BF16:
+        chunk_scale(static_cast<const __nv_bfloat16*>(t.src[i]), static_cast<__nv_bfloat16*>(t.dst[i]), t.count[i],
+                    chunk, chunks, single, coef);
+        break;
+      default:
+        chunk_scale(static_cast<const __half*>(t.src[i]), static_cast<__half*>(t.dst[i]), t.count[i], chunk, chunks,
+                    single, coef);
+        break;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+lewm_status clip_fail(lewm_status s, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  set_noctx_error(buf);
+  return s;
+}
+
+int64_t type_bytes(int32_t t) { return t == LEWM_TYPE_F32 ? 4 : 2; }
+
+struct GradList {
+  const void* const* src;
+  void* const* dst;  // or null: norm only
+  const int64_t* counts;
+  const int32_t* types;
+  int32_t n;
+};
+
+lewm_status check_list(const GradList& l, int32_t kind, const void* ws, const void* norm_out) {
+  if (l.n < 0) return clip_fail(LEWM_INVALID_ARG, "need n >= 0, got %d", l.n);
+  if (l.n > kMaxTensors) return clip_fail(LEWM_UNSUPPORTED_SHAPE, "%d tensors, at most %d", l.n, kMaxTensors);
+  if (kind != LEWM_NORM_L2 && kind != LEWM_NORM_MAX) return clip_fail(LEWM_INVALID_ARG, "unknown norm kind %d", kind);
+  if (!ws || !norm_out) return clip_fail(LEWM_INVALID_ARG, "workspace and norm_out must be non-NULL");
+  if (reinterpret_cast<uintptr_t>(ws) & 15) return clip_fail(LEWM_INVALID_ARG, "workspace must be 16-byte aligned");
+  if (l.n > 0 && (!l.src || !l.counts || !l.types))
+    return clip_fail(LEWM_INVALID_ARG, "src, counts and types must be non-NULL");
+  for (int32_t i = 0; i < l.n; ++i) {
+    if (l.types[i] < LEWM_TYPE_F32 || l.types[i] > LEWM_TYPE_F16)
+      return clip_fail(LEWM_INVALID_ARG, "tensor %d: unknown element type %d", i, l.types[i]);
+    if (l.counts[i] < 0) return clip_fail(LEWM_INVALID_ARG, "tensor %d: count must be >= 0", i);
+    // 2^45 bytes of chunks fit the table's 32-bit chunk numbers; no GPU holds as much.
+    if (l.counts[i] > (int64_t)1 << 42) return clip_fail(LEWM_UNSUPPORTED_SHAPE, "tensor %d: too many elements", i);
+    if (l.counts[i] == 0) continue;
+    const uintptr_t mask = type_bytes(l.types[i]) - 1;
+    if (!l.src[i] || (reinterpret_cast<uintptr_t>(l.src[i]) & mask))
+      return clip_fail(LEWM_INVALID_ARG, "tensor %d: NULL or misaligned pointer", i);
+    if (l.dst && (!l.dst[i] || (reinterpret_cast<uintptr_t>(l.dst[i]) & mask)))
+      return clip_fail(LEWM_INVALID_ARG, "tensor %d: NULL or misaligned destination", i);
+  }
+  return LEWM_OK;
+}
+
+// Fills `t` with the tensors from `from` on that fit; empty ones take no place. Returns the
+// index of the first tensor left.
+template <int N>
+int32_t fill_table(const GradList& l, int32_t from, Table<N>* t) {
+  t->n = 0;
+  uint64_t chunks = 0;
+  int32_t i = from;
+  for (; i < l.n && t->n < N; ++i) {
+    if (l.counts[i] == 0) continue;
+    const int64_t bytes = l.counts[i] * type_bytes(l.types[i]);
+    const uint64_t c = (uint64_t)((bytes + kChunkBytes - 1) / kChunkBytes);
+    if (chunks + c > 0xfffffff0ull) break;
+    const int k = t->n++;
+    t->src[k] = l.src[i];
+    t->dst[k] = l.dst ? l.dst[i] : nullptr;
+    t->count[k] = l.counts[i];
+    t->first[k] = (uint32_t)chunks;
+    const bool same = !l.dst || ((reinterpret_cast<uintptr_t>(l.src[i]) ^ reinterpret_cast<uintptr_t>(l.dst[i])) & 15) == 0;
+    t->kind[k] = (uint8_t)(l.types[i] | (same ? 0 : 4));
+    chunks += c;
+  }
+  t->first[t->n] = (uint32_t)chunks;
+  return i;
+}
+
+template <int N, bool MAX>
+cudaError_t run_norm(const GradList& l, double* part, int* slots, cudaStream_t st) {
+  Table<N> t;
+  *slots = 0;
+  for (int32_t i = 0; i < l.n;) {
+    i = fill_table(l, i, &t);
+    if (t.n == 0) continue;
+    const int32_t launches_left = (l.n - i + N - 1) / N;  // each gets its share of the slots
+    const int room = (kSlots - *slots) / (launches_left + 1);
+    const int grid = (int)std::min<uint32_t>(t.first[t.n], (uint32_t)std::min(kBlocks, room));
+    const cudaError_t e = launch_k(k_grad_norm<N, MAX>, dim3(grid), dim3(kThreads), 0, st, t, part + *slots);
+    if (e != cudaSuccess) return e;
+    *slots += grid;
+  }
+  return cudaSuccess;
+}
+
+template <int N, bool MAX>
+cudaError_t run_scale(const GradList& l, const double* part, int slots, const float* norm_in, float max_norm,
+                      float* norm_out, cudaStream_t st) {
+  Table<N> t;
+  int32_t i = 0;
+  do {
+    i = fill_table(l, i, &t);
+    int in_place = 1;
+    for (int k = 0; k < t.n; ++k) in_place &= t.src[k] == t.dst[k];
+    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(t.first[t.n], (uint32_t)kBlocks));
+    const cudaError_t e = launch_k(k_grad_scale<N, MAX>, dim3(grid), dim3(kThreads), 0, st, t, part, slots, norm_in,
+                                   max_norm, norm_out, in_place);
+    if (e != cudaSuccess) return e;
+  } while (i < l.n);
+  return cudaSuccess;
+}
+
+struct ClipDevice {
+  int prev = -1;
+  cudaError_t err = cudaSuccess;
+  explicit ClipDevice(int dev) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != dev) err = cudaSetDevice(dev);
+    else prev = -1;
+  }
+  ~ClipDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+template <int N, bool MAX>
+cudaError_t run_all(const GradList& l, float max_norm, const float* norm_in, void* ws, float* norm_out,
+                    cudaStream_t st) {
+  double* part = static_cast<double*>(ws);
+  int slots = 0;
+  if (!norm_in) {
+    const cudaError_t e = run_norm<N, MAX>(l, part, &slots, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (l.dst) return run_scale<N, MAX>(l, part, slots, norm_in, max_norm, norm_out, st);
+  return launch_k(k_norm_out<MAX>, dim3(1), dim3(kThreads), 0, st, (const double*)part, slots, norm_out);
+}
+
+lewm_status grad_call(const GradList& l, int32_t kind, float max_norm, const float* norm_in, void* ws, float* norm_out,
+                      int32_t device, void* stream) {
+  ClipDevice cd(device);
+  if (cd.err != cudaSuccess)
+    return clip_fail(LEWM_CUDA_ERROR, "cudaSetDevice(%d): %s", device, cudaGetErrorString(cd.err));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool mx = kind == LEWM_NORM_MAX;
+  // A short list takes the small table: parameters are copied on every launch.
+  const cudaError_t e =
+      l.n <= kSmall ? (mx ? run_all<kSmall, true>(l, max_norm, norm_in, ws, norm_out, st)
+                          : run_all<kSmall, false>(l, max_norm, norm_in, ws, norm_out, st))
+                    : (mx ? run_all<kLarge, true>(l, max_norm, norm_in, ws, norm_out, st)
+                          : run_all<kLarge, false>(l, max_norm, norm_in, ws, norm_out, st));
+  if (e != cudaSuccess) return clip_fail(LEWM_CUDA_ERROR, "gradient norm launch: %s", cudaGetErrorString(e));
+  return LEWM_OK;
+}
+
+}  // namespace
+}  // namespace lewm
+
+using namespace lewm;
+
+extern "C" lewm_status lewm_grad_norm(const void* const* src, const int64_t* counts, const int32_t* types, int32_t n,
+                                      int32_t kind, void* workspace, float* norm_out, int32_t device, void* stream) {
+  const GradList l{src, nullptr, counts, types, n};
+  const lewm_status s = check_list(l, kind, workspace, norm_out);
+  if (s != LEWM_OK) return s;
+  return grad_call(l, kind, 0.f, nullptr, workspace, norm_out, device, stream);
+}
+
+extern "C" lewm_status lewm_grad_clip(const void* const* src, void* const* dst, const int64_t* counts,
+                                      const int32_t* types, int32_t n, int32_t kind, float max_norm,
+                                      const float* norm_in, void* workspace, float* norm_out, int32_t device,
+                                      void* stream) {
+  if (n > 0 && !dst) return clip_fail(LEWM_INVALID_ARG, "dst must be non-NULL");
+  if (!(max_norm >= 0.f)) return clip_fail(LEWM_INVALID_ARG, "max_norm must be >= 0");
+  if (norm_in && norm_in == norm_out) return clip_fail(LEWM_INVALID_ARG, "norm_in and norm_out must differ");
+  void* none = nullptr;
+  const GradList l{src, n > 0 ? dst : &none, counts, types, n};
+  const lewm_status s = check_list(l, kind, workspace, norm_out);
+  if (s != LEWM_OK) return s;
+  return grad_call(l, kind, max_norm, norm_in, workspace, norm_out, device, stream);
+}

@@ -1,0 +1,533 @@
+"""Layer norm, adaptive layer norm, gradient norm and clipping on the GPU, against plain 64-bit
+forms within bounds derived in ``tests/training_reference.py``."""
+
+import copy
+import math
+
+import pytest
+import torch
+
+import lewm_flash_b200 as lf
+from tests.training_reference import (U, TinyPredictor, assert_within, half_step, norm_reference, sum_bound)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F16), (F16, F32), (F32, BF16)]
+TYPE_IDS = ["f32", "bf16-f32", "bf16", "f16", "f16-f32", "f32-bf16"]
+
+
+def randn(*shape, seed=0, scale=1.0, offset=0.0, dtype=F32):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, device=DEV, generator=g) * scale + offset).to(dtype)
+
+
+def activation(rows, width, dtype, seed=0):
+    x = randn(rows, width, seed=seed) * (0.2 + torch.arange(rows, device=DEV)[:, None] % 5)
+    x += randn(rows, 1, seed=seed + 1)
+    if rows > 3:
+        x[3] = 0.0
+    return x.to(dtype)
+
+
+def check_norm(x, a, b, eps, one_plus, group, y, dy, dx, da, db):
+    """All of a norm's outputs against the 64-bit form; a, b (groups, width) or None."""
+    width = x.shape[-1]
+    xf = x.detach().reshape(-1, width)
+    rows = xf.shape[0]
+
+    def per_row(p, default):
+        if p is None:
+            return torch.full((1, width), default, device=DEV)
+        p = p.detach().reshape(-1, width).double()
+        return p.repeat_interleave(group, 0) if p.shape[0] * group == rows and group else p
+
+    gain = per_row(a, 0.0 if one_plus else 1.0) + (1.0 if one_plus else 0.0)
+    ref = norm_reference(xf, gain, per_row(b, 0.0), eps, None if dy is None else dy.reshape(-1, width))
+    if one_plus:  # 1 + scale is rounded to float32
+        ref["e_y"] = ref["e_y"] + U * (ref["y"].abs() + per_row(b, 0.0).abs())
+    assert_within(y.reshape(-1, width), ref["y"], ref["e_y"], x.dtype, "y")
+    if dy is None:
+        return
+    if dx is not None:
+        if one_plus:
+            ref["e_dx"] = ref["e_dx"] * 1.5
+        assert_within(dx.reshape(-1, width), ref["dx"], ref["e_dx"], x.dtype, "dx")
+    n = group or rows
+    for got, p, e, what in ((da, ref["pz"], ref["e_pz"], "da"), (db, ref["p1"], torch.zeros_like(ref["p1"]), "db")):
+        if got is None:
+            continue
+        p, e = p.view(-1, n, width), e.view(-1, n, width)
+        assert_within(got.reshape(-1, width), p.sum(-2), sum_bound(p, e, n), got.dtype, what)
+
+
+SHAPES = [(1, 1), (1, 192), (3, 192), (2, 1), (5, 7), (33, 64), (900, 192), (257, 65), (130, 255), (131, 256), (70, 511),
+          (65, 512), (40, 1011), (301, 1024), (37, 2048), (20, 4097), (9, 8192), (5, 16384), (3, 16385), (299, 20001),
+          (5000, 40), (2500, 770)]
+
+
+@pytest.mark.parametrize("types", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("rows,width", SHAPES)
+def test_layer_norm_matches_64_bits(rows, width, types):
+    dtype, ptype = types
+    x = activation(rows, width, dtype).requires_grad_(True)
+    w = randn(width, seed=5, scale=0.2, offset=1.0, dtype=ptype).requires_grad_(True)
+    b = randn(width, seed=6, scale=0.2, dtype=ptype).requires_grad_(True)
+    dy = randn(rows, width, seed=7, scale=0.1, dtype=dtype)
+    y = lf.layer_norm(x, w, b)
+    assert y.dtype == dtype and y.shape == x.shape and y.is_contiguous()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert dw.dtype == ptype and db.dtype == ptype
+    check_norm(x, w, b, 1e-5, False, 0, y.detach(), dy, dx, dw, db)
+    with torch.no_grad():  # the form without statistics: the same bits
+        assert torch.equal(lf.layer_norm(x, w, b), y)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, F32), (F16, F16)], ids=["f32", "bf16-f32", "f16"])
+@pytest.mark.parametrize("batch,tokens,width", [(1, 1, 192), (300, 3, 192), (7, 5, 33), (400, 1, 96), (1000, 5, 70),
+                                                (300, 17, 1024), (2, 5000, 96), (9, 700, 1536), (64, 257, 384),
+                                                (3, 2, 16385), (40, 15, 2050)])
+@pytest.mark.parametrize("shared", [False, True], ids=["per_token", "per_sequence"])
+def test_ada_layer_norm_matches_64_bits(batch, tokens, width, shared, types):
+    dtype, ctype = types
+    x = activation(batch * tokens, width, dtype).view(batch, tokens, width).requires_grad_(True)
+    mod = randn(batch, 1 if shared else tokens, 3 * width, seed=3, scale=0.4, dtype=ctype)
+    shift, scale, _ = (t.requires_grad_(True) for t in mod.chunk(3, -1))
+    dy = randn(batch, tokens, width, seed=7, scale=0.1, dtype=dtype)
+    y = lf.ada_layer_norm(x, shift, scale)
+    dx, dshift, dscale = torch.autograd.grad(y, (x, shift, scale), dy)
+    assert dshift.shape == shift.shape and dscale.dtype == ctype
+    check_norm(x, scale, shift, 1e-6, True, tokens if shared else 1, y.detach(), dy, dx, dscale, dshift)
+
+
+@pytest.mark.parametrize("shape,mod", [((4, 6, 3, 32), (4, 1, 1, 32)), ((4, 6, 3, 32), (4, 6, 1, 32)),
+                                       ((4, 6, 3, 32), (32,)), ((4, 6, 3, 32), (1, 1, 1, 32)), ((6, 32), (6, 32)),
+                                       ((1, 6, 32), (6, 32)), ((1, 32), (32,)), ((32,), (32,)), ((5, 1, 32), (5, 1, 32))])
+def test_ada_modulation_shapes(shape, mod):
+    x = randn(*shape, seed=1).requires_grad_(True)
+    shift = randn(*mod, seed=2, scale=0.3).requires_grad_(True)
+    scale = randn(*mod, seed=3, scale=0.3).requires_grad_(True)
+    dy = randn(*shape, seed=4)
+    y = lf.ada_layer_norm(x, shift, scale)
+    dx, dshift, dscale = torch.autograd.grad(y, (x, shift, scale), dy)
+    rows = x.numel() // 32
+    check_norm(x, scale, shift, 1e-6, True, rows // (shift.numel() // 32), y.detach(), dy, dx, dscale, dshift)
+    assert dshift.shape == shift.shape and dscale.shape == scale.shape
+
+
+@pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("rows,width", [(3, 192), (1300, 192), (20, 20000)])
+def test_layer_norm_without_weight_or_bias(rows, width, weight, bias):
+    x = activation(rows, width, F32).requires_grad_(True)
+    w = randn(width, seed=5, scale=0.2, offset=1.0).requires_grad_(True) if weight else None
+    b = randn(width, seed=6, scale=0.2).requires_grad_(True) if bias else None
+    dy = randn(rows, width, seed=7)
+    y = lf.layer_norm(x, w, b, eps=1e-3)
+    leaves = [t for t in (x, w, b) if t is not None]
+    grads = dict(zip([id(t) for t in leaves], torch.autograd.grad(y, leaves, dy)))
+    check_norm(x, w, b, 1e-3, False, 0, y.detach(), dy, grads[id(x)], grads.get(id(w)), grads.get(id(b)))
+
+
+@pytest.mark.parametrize("need", [(True, False, False), (False, True, False), (False, False, True), (False, True, True),
+                                  (True, False, True)])
+@pytest.mark.parametrize("rows,width", [(3, 192), (1300, 192), (1300, 700), (20, 20000)])
+def test_only_the_wanted_gradients(rows, width, need):
+    ts = [activation(rows, width, F32), randn(width, seed=5), randn(width, seed=6)]
+    for t, n in zip(ts, need):
+        t.requires_grad_(n)
+    dy = randn(rows, width, seed=7)
+    y = lf.layer_norm(*ts)
+    got = iter(torch.autograd.grad(y, [t for t, n in zip(ts, need) if n], dy))
+    check_norm(*ts, 1e-5, False, 0, y.detach(), dy, *[next(got) if n else None for n in need])
+
+
+@pytest.mark.parametrize("make", [
+    lambda t: t[:, 1:193], lambda t: t[:, 3:196], lambda t: t[::2, :192], lambda t: t[5:6, :192].expand(40, 192),
+    lambda t: t[:192].t(), lambda t: t[:, :192].unflatten(0, (20, 2))[:, :1], lambda t: t[:, :1],
+    lambda t: t[:, :192].unflatten(0, (4, 10))[:, :3], lambda t: t[3, 8:200],
+], ids=["offset1", "odd", "every_second", "expanded", "transposed", "even_steps", "one_column", "uneven", "vector"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strided_inputs(make, dtype):
+    base = randn(40, 256, seed=1, dtype=dtype)
+    if make(base[:, :]).shape[-1] == 40:
+        base = randn(192, 40, seed=1, dtype=dtype)
+    x = make(base).detach().requires_grad_(True)
+    n = x.shape[-1]
+    w, b = randn(2 * n, seed=2)[::2].requires_grad_(True), randn(n, seed=3).requires_grad_(True)
+    wide = randn(*x.shape[:-1], n + 7, seed=4, dtype=dtype)
+    dy = wide[..., 2:n + 2]
+    y = lf.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    check_norm(x, w, b, 1e-5, False, 0, y.detach(), dy, dx, dw, db)
+
+
+def test_expanded_output_gradient():
+    x = randn(33, 192, seed=1).requires_grad_(True)
+    w = randn(192, seed=2).requires_grad_(True)
+    y = lf.layer_norm(x, w)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w))
+    check_norm(x, w, None, 1e-5, False, 0, y.detach(), torch.ones_like(x), dx, dw, None)
+
+
+@pytest.mark.parametrize("shape", [(0, 192), (3, 0, 64)])
+def test_no_rows(shape):
+    x = torch.zeros(*shape, device=DEV, requires_grad=True)
+    w = torch.ones(shape[-1], device=DEV, requires_grad=True)
+    b = torch.ones(shape[-1], device=DEV, requires_grad=True)
+    y = lf.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == x.shape == dx.shape and not dw.any() and not db.any()
+    y = lf.ada_layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == x.shape == dx.shape and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("width", [40, 192, 700, 20000])
+def test_nonfinite_rows_stay_in_their_row(bad, width):
+    x = activation(50, width, F32)
+    w, b, dy = randn(width, seed=2), randn(width, seed=3), randn(50, width, seed=4)
+    clean_x = x.clone().requires_grad_(True)
+    x[17, width // 2] = bad
+    x.requires_grad_(True)
+    y, yc = lf.layer_norm(x, w, b), lf.layer_norm(clean_x, w, b)
+    (dx,), (dxc,) = torch.autograd.grad(y, x, dy), torch.autograd.grad(yc, clean_x, dy)
+    others = torch.arange(50, device=DEV) != 17
+    assert y[17].isnan().all() and dx[17].isnan().all()
+    assert torch.equal(y[others], yc[others]) and torch.equal(dx[others], dxc[others])
+
+
+def test_large_offset_keeps_the_variance():
+    x = randn(64, 384, seed=1, scale=1e-2, offset=100.0).requires_grad_(True)
+    dy = randn(64, 384, seed=2)
+    y = lf.layer_norm(x)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    check_norm(x, None, None, 1e-5, False, 0, y.detach(), dy, dx, None, None)
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the 64-bit forward, central differences: step h leaves h^2 / 6 of a
+    third derivative of order 10, so 1e-6 at h = 1e-4 is far under the float32 gradients' 1e-5."""
+    torch.manual_seed(0)
+    x, shift, scale = randn(6, 4, 48, seed=1), randn(6, 1, 48, seed=2), randn(6, 1, 48, seed=3)
+    dy = randn(6, 4, 48, seed=4)
+    leaves = [t.requires_grad_(True) for t in (x, shift, scale)]
+    grads = torch.autograd.grad(lf.ada_layer_norm(*leaves), leaves, dy)
+
+    def f(x, shift, scale):
+        mu = x.mean(-1, keepdim=True)
+        v = ((x - mu) ** 2).mean(-1, keepdim=True)
+        return (((x - mu) / torch.sqrt(v + 1e-6) * (1 + scale) + shift) * dy.double()).sum()
+
+    args = [t.detach().double() for t in leaves]
+    for i, g in enumerate(grads):
+        v = torch.randn_like(args[i])
+        h = 1e-4
+        up = f(*[t + h * v if j == i else t for j, t in enumerate(args)])
+        down = f(*[t - h * v if j == i else t for j, t in enumerate(args)])
+        want, got = float((up - down) / (2 * h)), float((g.double() * v).sum())
+        assert abs(got - want) <= 1e-5 * float((g.double() * v).abs().sum())
+
+
+def test_results_do_not_depend_on_the_run():
+    x = activation(4099, 700, BF16).requires_grad_(True)
+    w, b = randn(700, seed=2).requires_grad_(True), randn(700, seed=3).requires_grad_(True)
+    dy = randn(4099, 700, seed=4, dtype=BF16)
+    runs = [torch.autograd.grad(lf.layer_norm(x, w, b), (x, w, b), dy) for _ in range(4)]
+    for r in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(r, runs[0]))
+    grads = [randn(n, seed=n) for n in (5, 70001, 333, 1 << 20)]
+    norms = [lf.grad_norm(grads) for _ in range(4)]
+    assert all(torch.equal(n, norms[0]) for n in norms)
+
+
+def test_double_backward_is_refused():
+    x = randn(4, 32).requires_grad_(True)
+    (g,) = torch.autograd.grad(lf.layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_input_changed_in_place_before_backward_is_refused():
+    x = randn(4, 32).requires_grad_(True)
+    h = x * 2
+    y = lf.layer_norm(h)
+    h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_side_stream_and_two_calls_at_once():
+    """Passes on two streams at the same time: each has its own workspace."""
+    x = activation(3000, 192, F32)
+    w, b, dy = randn(192, seed=2), randn(192, seed=3), randn(3000, 192, seed=4)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(lf.layer_norm(*leaves), leaves, dy)
+    want_norm = lf.grad_norm(want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            g = torch.autograd.grad(lf.layer_norm(*leaves), leaves, dy)
+            got.append((g, lf.grad_norm(g)))
+    torch.cuda.synchronize()
+    for g, n in got:
+        assert all(torch.equal(p, q) for p, q in zip(g, want)) and torch.equal(n, want_norm)
+
+
+def test_captured_training_pass_replays_on_new_inputs():
+    """Forward, backward and clip in one graph; two graphs of it replayed at the same time."""
+    x = activation(900, 192, F32)
+    w, b, dy = randn(192, seed=2), randn(192, seed=3), randn(900, 192, seed=4)
+
+    def step(x, w, b, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        grads = torch.autograd.grad(lf.layer_norm(*leaves), leaves, dy)
+        return lf.clip_grads(grads, 0.5)
+
+    s = torch.cuda.Stream(DEV)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(x, w, b, dy)
+    torch.cuda.current_stream().wait_stream(s)
+    runs = []
+    for k in range(2):
+        sx, sdy = x.clone(), dy.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(sx, w, b, sdy)
+        runs.append((graph, sx, sdy, out))
+    for seed in (11, 12):
+        for k, (graph, sx, sdy, out) in enumerate(runs):
+            sx.copy_(activation(900, 192, F32, seed=seed + 10 * k))
+            sdy.copy_(randn(900, 192, seed=seed + 10 * k + 5))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream(DEV) for _ in runs]
+        for st, (graph, *_) in zip(streams, runs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, sx, sdy, out in runs:
+            want, norm = step(sx, w, b, sdy)
+            assert torch.equal(out[1], norm) and all(torch.equal(p, q) for p, q in zip(out[0], want))
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements; the last rows and the parameter gradients are checked."""
+    rows, width = (1 << 31) // 2048 + 5, 2048
+    x = torch.zeros(rows, width, device=DEV, dtype=BF16)
+    dy = torch.zeros_like(x)
+    x[-3:] = activation(3, width, BF16)
+    dy[-3:] = randn(3, width, seed=4, dtype=BF16)
+    x.requires_grad_(True)
+    w, b = randn(width, seed=2).requires_grad_(True), randn(width, seed=3).requires_grad_(True)
+    y = lf.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    check_norm(x.detach()[-3:], w, b, 1e-5, False, 0, y.detach()[-3:], dy[-3:], dx[-3:], dw, db)
+    assert torch.equal(y[:2].detach(), b.detach().to(BF16).expand(2, -1)) and not dx[:-3].any()
+    clipped, norm = lf.clip_grads([dy.view(-1)[1:]], 1.0)
+    want = dy[-3:].double().norm()
+    assert abs(norm.double() - want) <= 8 * U * want
+    assert_within(clipped[0][-3 * width:], dy[-3:].double().view(-1) / want,
+                  dy[-3:].double().abs().view(-1) / want * 12 * U, BF16)
+
+
+# ---------------------------------------------------------------------------- gradient norm, clipping
+def gradients(sizes, kinds, scale=1.0, offset=0):
+    """Tensors of the sizes, types in turn, each `offset` elements into its own allocation."""
+    return [randn(n + offset, seed=i, scale=scale * 10.0 ** -(i % 3), dtype=kinds[i % len(kinds)])[offset:]
+            for i, n in enumerate(sizes)]
+
+
+def norm64(grads, kind=2.0):
+    if kind == math.inf:
+        return max([float(g.double().abs().max()) for g in grads if g.numel()], default=0.0)
+    return math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+
+
+def check_clip(before, after, norm, max_norm, kind=2.0):
+    """norm: sums of 8 products are 8 roundings, the root halves them, one to float32: 5 u. factor: the
+    added 1e-6 and the quotient, 2 u more; the product, 1 u."""
+    want = norm64(before, kind)
+    assert norm.dtype == F32 and norm.shape == () and abs(float(norm) - want) <= 6 * U * want
+    coef = min(1.0, max_norm / (want + 1e-6))
+    for b, a in zip(before, after):
+        assert a.dtype == b.dtype and a.shape == b.shape
+        assert_within(a, b.double() * coef, b.double().abs() * coef * 10 * U, b.dtype, "clipped")
+
+
+SIZES = {"one": [1], "vector": [1500], "odd": [3, 1, 17, 1023, 4096, 4097, 8191, 70001],
+         "empty_among": [0, 5, 0, 0, 9000, 0], "64": [100 + i for i in range(64)], "65": [100 + i for i in range(65)],
+         "1500": [1 + 37 * (i % 29) for i in range(1500)], "large": [5000011, 3, 1 << 22]}
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("kinds", [[F32], [BF16], [F16], [F32, BF16, F16]], ids=["f32", "bf16", "f16", "mixed"])
+@pytest.mark.parametrize("sizes", list(SIZES.values()), ids=list(SIZES))
+def test_norm_and_clip_match_64_bits(sizes, kinds, kind):
+    grads = gradients(sizes, kinds, scale=4.0)
+    before = [g.clone() for g in grads]
+    norm = lf.grad_norm(grads, kind)
+    want = norm64(before, kind)
+    assert abs(float(norm) - want) <= 6 * U * want
+    for max_norm in (0.37 * want, 2.0 * want + 1.0):
+        clipped, n2 = lf.clip_grads(grads, max_norm, kind)
+        assert torch.equal(n2, norm) and all(torch.equal(g, b) for g, b in zip(grads, before))
+        check_clip(before, clipped, n2, max_norm, kind)
+    params = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    n3 = lf.clip_grad_norm_(params, 0.37 * want, kind)
+    assert torch.equal(n3, norm) and all(p.grad is g for p, g in zip(params, grads))
+    check_clip(before, grads, n3, 0.37 * want, kind)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("src_off,dst_off", [(1, 1), (3, 3), (0, 1), (5, 2), (7, 0)])
+def test_unaligned_tensors(dtype, src_off, dst_off):
+    """Sources and destinations at the same and at different offsets from 16 bytes; nothing else is written."""
+    sizes = [1, 2, 9, 4099, 20011]
+    grads = gradients(sizes, [dtype], offset=src_off)
+    bufs = [torch.full((n + dst_off + 9,), 7.0, device=DEV, dtype=dtype) for n in sizes]
+    out = [t[dst_off:dst_off + n] for t, n in zip(bufs, sizes)]
+    got, norm = lf.clip_grads(grads, 0.5, out=out)
+    assert all(g is o for g, o in zip(got, out))
+    check_clip(grads, out, norm, 0.5)
+    for t, n in zip(bufs, sizes):
+        assert (t[:dst_off] == 7.0).all() and (t[dst_off + n:] == 7.0).all()
+
+
+def test_factor_one_keeps_the_bits():
+    g = [torch.tensor([1.0, -0.0, 1e-42, 3e-39], device=DEV), randn(1000, dtype=BF16)]
+    before = [t.clone() for t in g]
+    for max_norm in (1e9, math.inf):
+        out, _ = lf.clip_grads(g, max_norm)
+        lf.clip_grads(g, max_norm, out=g)
+        for t, o, b in zip(g, out, before):
+            assert torch.equal(t.view(torch.int16), b.view(torch.int16))
+            assert torch.equal(o.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("scale", [1e30, 1e-30, 1e18, 1e-20])
+def test_squares_beyond_float32(scale):
+    grads = [randn(5000, seed=1) * scale, torch.zeros(100, device=DEV), randn(77, seed=2) * scale]
+    want = norm64(grads)
+    norm = lf.grad_norm(grads)
+    assert abs(float(norm) - want) <= 6 * U * want
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+def test_nonfinite_gradients(bad, kind):
+    grads = gradients([300, 5001], [F32, BF16])
+    grads[1][4321] = bad
+    norm = lf.grad_norm(grads, kind)
+    assert norm.isnan() if math.isnan(bad) else norm == math.inf
+    params = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    before = [g.clone() for g in grads]
+    with pytest.raises(RuntimeError, match="non-finite"):
+        lf.clip_grad_norm_(params, 1.0, kind, error_if_nonfinite=True)
+    assert all(torch.equal(g.view(torch.int16), b.view(torch.int16)) for g, b in zip(grads, before))
+    lf.clip_grad_norm_(params, 1.0, kind)
+    if math.isnan(bad):
+        assert all(g.isnan().all() for g in grads)
+    else:  # a factor of 0: zeros, and infinity times 0 is NaN
+        assert grads[1][4321].isnan() and not grads[0].any()
+
+
+def test_max_norm_zero_and_zero_gradients():
+    grads = gradients([300, 5001], [F32, BF16])
+    out, _ = lf.clip_grads(grads, 0.0)
+    assert not any(t.any() for t in out)
+    zeros = [torch.zeros(1000, device=DEV), torch.zeros(0, device=DEV)]
+    out, norm = lf.clip_grads(zeros, 1.0)
+    assert norm == 0.0 and not out[0].any()
+    assert lf.grad_norm([torch.zeros(0, device=DEV)]) == 0.0
+
+
+def test_clip_in_place_matches_torch_and_finite_checks_pass():
+    grads = gradients([300, 5001, 64], [F32])
+    mine = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    theirs = [torch.nn.Parameter(torch.empty_like(g)) for g in grads]
+    for a, b, g in zip(mine, theirs, grads):
+        a.grad, b.grad = g.clone(), g.clone()
+    n1 = lf.clip_grad_norm_(mine, 0.9, error_if_nonfinite=True)
+    n2 = torch.nn.utils.clip_grad_norm_(theirs, 0.9, error_if_nonfinite=True)
+    torch.testing.assert_close(n1, n2, rtol=2e-6, atol=0)
+    for a, b in zip(mine, theirs):
+        torch.testing.assert_close(a.grad, b.grad, rtol=4e-6, atol=0)
+
+
+def test_strided_gradients_are_clipped_in_place():
+    base = randn(40, 60, seed=3)
+    before = base.clone()
+    p, q = torch.nn.Parameter(torch.empty(40, 10, device=DEV)), torch.nn.Parameter(torch.empty(30, 40, device=DEV))
+    p.grad, q.grad = base[:, 5:15], base[:, 20:50].t()
+    want = [p.grad.clone(), q.grad.clone()]
+    norm = lf.clip_grad_norm_([p, q], 0.7)
+    check_clip(want, [p.grad, q.grad], norm, 0.7)
+    untouched = torch.ones(60, dtype=torch.bool, device=DEV)
+    untouched[5:15] = untouched[20:50] = False
+    assert torch.equal(base[:, untouched], before[:, untouched])
+    with pytest.raises(ValueError, match="overlap"):
+        lf.clip_grad_norm_([p, p], 0.7)
+
+
+def test_clipping_counts_as_a_change_in_place():
+    w = randn(64, seed=1).requires_grad_(True)
+    h = w * 1.0
+    loss = h.square().sum()  # saves h
+    d = h.detach()
+    lf.clip_grads([d], 0.1, out=[d])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+# ---------------------------------------------------------------------------- together
+@pytest.mark.parametrize("mode", ["float32", "autocast"])
+def test_training_step_of_a_predictor_with_installed_norms(mode):
+    """Forward, backward and clip of a small AdaLN predictor with its norms routed, against the same
+    model in float64. A float32 layer has about 10 chained operations of up to 56 u relative error, so
+    2 layers forward and back stay within 40 x 56 u = 1.4e-4 of each gradient's largest element. Under
+    bf16 autocast the products round their operands to 2^-9 relative; torch's own autocast run is the
+    measure there: no more than twice its error plus one rounding."""
+    torch.manual_seed(0)
+    model = TinyPredictor().to(DEV)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(0.05 * torch.randn_like(p))
+    x, c, target = randn(30, 3, 64, seed=1), randn(30, 3, 64, seed=2), randn(30, 3, 64, seed=3)
+
+    def grads_of(m, dtype, autocast):
+        m.zero_grad(set_to_none=True)
+        with torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+            y = m(x.to(dtype), c.to(dtype))
+        ((y.to(dtype) - target.to(dtype)) ** 2).mean().backward()
+        return {n: p.grad.double() for n, p in m.named_parameters()}
+
+    exact = grads_of(copy.deepcopy(model).double(), torch.float64, False)
+    plain = grads_of(copy.deepcopy(model), F32, mode == "autocast")
+    handle = lf.install_training_norms(model)
+    assert len(handle.modules) == 2 * 5 + 1  # a block and its four norms, twice, and the last norm
+    got = grads_of(model, F32, mode == "autocast")
+    for n, want in exact.items():
+        top = float(want.abs().max())
+        err = float((got[n] - want).abs().max())
+        if mode == "float32":
+            assert err <= 40 * 56 * U * top, n
+        else:
+            assert err <= 2 * float((plain[n] - want).abs().max()) + half_step(BF16) * top, n
+    before = [p.grad.clone() for p in model.parameters()]
+    norm = lf.clip_grad_norm_(model.parameters(), 0.01)
+    check_clip(before, [p.grad for p in model.parameters()], norm, 0.01)
+    torch.optim.SGD(model.parameters(), lr=0.1).step()
+    clone = copy.deepcopy(model)  # a copy's routed modules use its own parameters
+    with torch.no_grad():
+        for p in clone.parameters():
+            p.zero_()
+        assert not clone(x, c).any() and model(x, c).any()
+    handle.remove()
+    assert all("forward" not in m.__dict__ for m in model.modules())
