@@ -1,0 +1,454 @@
+// The training operators as torch functions: argument checks, strides, allocation, streams and
+// autograd around the C ABI of lewm_b200.h (lewm_norm_*, lewm_grad_*), as the Python extension
+// module lewm_flash_b200._torch_ops. lewm_flash_b200/training.py is the documented surface.
+//
+// In C++ because a training step calls these operators a hundred times on rows that take the GPU
+// a few microseconds. Host time of a forward and backward pass (900 x 192 float32): through a
+// Python autograd.Function and ctypes 140 us, through this module's autograd node 62 us (45 of
+// them the autograd engine's own); a forward pass alone 15 and 4 us; a clip of 523 tensors, with
+// its checks, 677 and 102 us.
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/utils/pybind.h>
+#include <ATen/ATen.h>
+
+#include <algorithm>
+#include <cmath>
+#include <limits>
+#include <optional>
+#include <vector>
+
+#include "lewm_b200.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+namespace {
+
+// ------------------------------------------------------------------ checks
+int type_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return LEWM_TYPE_F32;
+    case at::kBFloat16: return LEWM_TYPE_BF16;
+    case at::kHalf: return LEWM_TYPE_F16;
+    default: return -1;
+  }
+}
+
+void check_tensor(const char* name, const Tensor& t) {
+  TORCH_CHECK_VALUE(type_code(t) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor, got layout ", t.layout());
+}
+
+void check_same_device(const char* name, const Tensor& t, const Tensor& x) {
+  TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", x on ", x.device());
+}
+
+void need_cuda(const Tensor& t) {
+  TORCH_CHECK_VALUE(t.is_cuda(), "the B200 training operators need a CUDA device, got ", t.device());
+}
+
+float check_eps(double eps) {
+  TORCH_CHECK_VALUE(eps >= 0.0 && eps < std::numeric_limits<double>::infinity(), "eps must be finite and >= 0, got ",
+                    eps);
+  return static_cast<float>(eps);
+}
+
+// Raises the package's LewmError for a failed C-ABI call made with the GIL held; in a backward pass
+// (an engine thread) the error becomes a RuntimeError with the same text.
+void check_status(lewm_status s, bool in_backward = false) {
+  if (s == LEWM_OK) return;
+  const char* msg = lewm_last_error(nullptr);
+  TORCH_CHECK(!in_backward, "lewm_b200 status ", static_cast<int>(s), ": ", msg);
+  py::object lib = py::module_::import("lewm_flash_b200._lib");
+  py::object type = lib.attr(s == LEWM_INVALID_ARG ? "LewmInvalidArgument" : "LewmError");
+  PyErr_SetObject(type.ptr(), type(static_cast<int>(s), msg).ptr());
+  throw py::error_already_set();
+}
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// ------------------------------------------------------------------ rows
+struct Rows {
+  Tensor t;
+  int64_t stride;
+};
+
+// `t` as rows of its last dim and the elements between them, copied only where the leading dims do
+// not step evenly through memory or the last dim is not dense.
+Rows rows_of(const Tensor& t) {
+  const auto size = t.sizes(), stride = t.strides();
+  const int64_t last = t.dim() - 1;
+  if (t.is_contiguous()) return {t, size[last]};
+  if (stride[last] == 1 || size[last] == 1) {
+    int64_t step = -1, extent = 1;  // stride of the rows so far, and how many there are
+    bool even = true;
+    for (int64_t d = last - 1; d >= 0 && even; --d) {
+      if (size[d] == 1) continue;
+      if (step < 0) step = stride[d];
+      else even = stride[d] == step * extent;
+      extent *= size[d];
+    }
+    if (even) return {t, step < 0 ? size[last] : step};
+  }
+  return {t.contiguous(), size[last]};
+}
+
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+// ------------------------------------------------------------------ norms
+// y = z a + b (group 0) or z (1 + a) + b with a row of a and b for `group` rows of x. x is `rows_of`.
+Tensor norm_forward(const Rows& x, const Tensor& a, const Tensor& b, float eps, int64_t group, float* stats) {
+  const int64_t width = x.t.size(-1), rows = x.t.numel() / width;
+  Tensor y = at::empty(x.t.sizes(), x.t.options().memory_format(at::MemoryFormat::Contiguous));
+  if (rows == 0) return y;
+  const Rows ra = a.defined() ? rows_of(a) : Rows{}, rb = b.defined() ? rows_of(b) : Rows{};
+  const int p_type = a.defined() ? type_code(a) : b.defined() ? type_code(b) : LEWM_TYPE_F32;
+  const lewm_norm_desc d{rows, width, x.stride, group, ra.stride, rb.stride, type_code(x.t), p_type, eps};
+  check_status(lewm_norm_forward(&d, x.t.const_data_ptr(), ptr(ra.t), ptr(rb.t), y.mutable_data_ptr(), stats,
+                                 x.t.get_device(), stream_of(x.t)));
+  return y;
+}
+
+struct NormBackward : public torch::autograd::Node {
+  SavedVariable x_, a_;
+  Tensor stats_;
+  float eps = 0.f;
+  int64_t group = 0;
+  std::vector<int64_t> x_shape, a_shape, b_shape;
+  at::ScalarType p_type = at::kFloat;
+  bool has_a = false, has_b = false;
+
+  std::string name() const override { return "LewmNormBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x_.reset_data();
+    a_.reset_data();
+    stats_.reset();
+  }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(3);
+    Tensor dy = grads[0];
+    const bool need_x = task_should_compute_output(0), need_a = has_a && task_should_compute_output(1),
+               need_b = has_b && task_should_compute_output(2);
+    if (!dy.defined() || !(need_x || need_a || need_b)) return out;
+    Tensor x, a, stats;
+    {
+      std::lock_guard<std::mutex> lock(mutex_);
+      x = x_.unpack();
+      if (has_a) a = a_.unpack();
+      stats = stats_;
+    }
+    const bool twice = at::GradMode::is_enabled();  // create_graph: a second pass would need our derivative
+    {
+      at::NoGradGuard no_grad;
+      const int64_t width = x_shape.back(), rows = x.numel() / width;
+      const auto opt = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
+      if (need_x) out[0] = at::empty(x_shape, opt);
+      // A shift row per row of x: its gradient is dy.
+      const bool dy_is_db = need_b && group == 1 && rows > 0 && p_type == dy.scalar_type();
+      if (rows == 0) {
+        if (need_a) out[1] = at::zeros(a_shape, opt.dtype(p_type));
+        if (need_b) out[2] = at::zeros(b_shape, opt.dtype(p_type));
+      } else {
+        if (need_a) out[1] = at::empty(a_shape, opt.dtype(p_type));
+        if (need_b && !dy_is_db) out[2] = at::empty(b_shape, opt.dtype(p_type));
+        if (need_x || need_a || out[2].defined()) {
+          const Rows rx = rows_of(x), rd = rows_of(dy), ra = a.defined() ? rows_of(a) : Rows{};
+          const int p = p_type == at::kFloat ? LEWM_TYPE_F32 : p_type == at::kBFloat16 ? LEWM_TYPE_BF16 : LEWM_TYPE_F16;
+          const lewm_norm_desc d{rows, width, rx.stride, group, ra.stride, 0, type_code(x), p, eps};
+          const size_t bytes = need_a || out[2].defined() ? lewm_norm_workspace(&d) : 0;
+          Tensor ws;
+          if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, opt.dtype(at::kByte));
+          check_status(lewm_norm_backward(&d, rd.t.const_data_ptr(), rd.stride, rx.t.const_data_ptr(), ptr(ra.t),
+                                          static_cast<const float*>(stats.const_data_ptr()), mut(out[0]), mut(out[1]),
+                                          mut(out[2]), mut(ws), bytes, x.get_device(), stream_of(x)),
+                       true);
+        }
+        if (dy_is_db) out[2] = dy.detach().reshape(b_shape);
+      }
+    }
+    if (twice) {
+      variable_list defined;
+      for (auto& t : out)
+        if (t.defined()) defined.push_back(t.detach().requires_grad_(true));
+      auto error = std::make_shared<torch::autograd::DelayedError>(
+          "the B200 norms are differentiable once: their gradients cannot be differentiated", defined.size());
+      defined = (*error)(std::move(defined));
+      size_t i = 0;
+      for (auto& t : out)
+        if (t.defined()) t = defined[i++];
+    }
+    return out;
+  }
+};
+
+Tensor norm(const Tensor& x, const Tensor& a, const Tensor& b, float eps, int64_t group) {
+  need_cuda(x);
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (a.defined() && a.requires_grad()) ||
+                                                   (b.defined() && b.requires_grad()));
+  if (!grad) {
+    at::NoGradGuard no_grad;
+    return norm_forward(rows_of(x), a, b, eps, group, nullptr);
+  }
+  auto node = std::shared_ptr<NormBackward>(new NormBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, a, b));
+  Tensor y;
+  {
+    at::NoGradGuard no_grad;
+    const Rows rx = rows_of(x);  // a copy, where one is needed, serves the backward pass too
+    const int64_t rows = x.numel() / x.size(-1);
+    node->stats_ = at::empty({2, rows}, x.options().dtype(at::kFloat).requires_grad(false));
+    y = norm_forward(rx, a, b, eps, group, static_cast<float*>(node->stats_.mutable_data_ptr()));
+    node->x_ = SavedVariable(rx.t, false);
+    if (a.defined()) node->a_ = SavedVariable(a, false);
+  }
+  node->eps = eps;
+  node->group = group;
+  node->x_shape = x.sizes().vec();
+  node->has_a = a.defined();
+  node->has_b = b.defined();
+  if (a.defined()) node->a_shape = a.sizes().vec(), node->p_type = a.scalar_type();
+  if (b.defined()) node->b_shape = b.sizes().vec(), node->p_type = b.scalar_type();
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
+Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+  check_tensor("x", x);
+  TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last dim of at least 1, got shape ", x.sizes());
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  auto check_param = [&](const char* name, const Tensor& p) {
+    if (!p.defined()) return;
+    check_tensor(name, p);
+    check_same_device(name, p, x);
+    TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == x.size(-1), name, " must be (", x.size(-1), ",), got ", p.sizes());
+  };
+  check_param("weight", w);
+  check_param("bias", b);
+  if (w.defined() && b.defined())
+    TORCH_CHECK_VALUE(w.scalar_type() == b.scalar_type(), "weight and bias must have one type, got ", w.scalar_type(),
+                      " and ", b.scalar_type());
+  return norm(x, w, b, check_eps(eps), 0);
+}
+
+Tensor ada_layer_norm(const Tensor& x, const Tensor& shift, const Tensor& scale, double eps) {
+  check_tensor("x", x);
+  TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last dim of at least 1, got shape ", x.sizes());
+  check_tensor("shift", shift);
+  check_tensor("scale", scale);
+  check_same_device("shift", shift, x);
+  check_same_device("scale", scale, x);
+  TORCH_CHECK_VALUE(shift.sizes() == scale.sizes() && shift.scalar_type() == scale.scalar_type(),
+                    "shift and scale must have one shape and type, got ", shift.sizes(), " ", shift.scalar_type(),
+                    " and ", scale.sizes(), " ", scale.scalar_type());
+  int64_t group = 1;
+  if (shift.sizes() != x.sizes()) {
+    const int64_t n = x.dim(), pad = n - shift.dim();
+    auto m = [&](int64_t d) { return d < pad ? int64_t{1} : shift.size(d - pad); };
+    bool fits = pad >= 0 && shift.dim() > 0 && shift.size(-1) == x.size(-1);
+    int64_t d = n - 2;
+    for (; fits && d >= 0 && m(d) == 1; --d) group *= x.size(d);
+    for (; fits && d >= 0; --d) fits = m(d) == x.size(d);
+    TORCH_CHECK_VALUE(fits, "shift and scale of shape ", shift.sizes(), " do not modulate x of shape ", x.sizes(),
+                      ": give a row per row of x, or size 1 in the dims before the last");
+  }
+  if (x.numel() == 0) group = 1;  // no rows
+  return norm(x, scale, shift, check_eps(eps), group);
+}
+
+// ------------------------------------------------------------------ gradient norm and clipping
+int norm_kind(double norm_type) {
+  if (norm_type == 2.0) return LEWM_NORM_L2;
+  TORCH_CHECK_VALUE(norm_type == std::numeric_limits<double>::infinity(), "norm_type must be 2 or inf, got ",
+                    norm_type);
+  return LEWM_NORM_MAX;
+}
+
+float check_max_norm(double max_norm) {
+  TORCH_CHECK_VALUE(max_norm >= 0.0, "max_norm must be >= 0, got ", max_norm);
+  return static_cast<float>(max_norm);
+}
+
+void check_list(const char* name, const std::vector<Tensor>& ts) {
+  for (size_t i = 0; i < ts.size(); ++i) {
+    const Tensor& t = ts[i];
+    if (type_code(t) < 0 || t.layout() != at::kStrided)
+      check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
+    TORCH_CHECK_VALUE(t.device() == ts[0].device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
+                      ts[0].device(), ": one device per call");
+  }
+}
+
+// Whether any destination [dst, dst + size) meets another destination or another tensor's source.
+bool overlap(const std::vector<int64_t>& src, const std::vector<int64_t>& dst, const std::vector<int64_t>& size) {
+  std::vector<std::pair<int64_t, int64_t>> out;
+  out.reserve(dst.size());
+  for (size_t i = 0; i < dst.size(); ++i)
+    if (size[i] > 0) out.emplace_back(dst[i], dst[i] + size[i]);
+  std::sort(out.begin(), out.end());
+  for (size_t i = 1; i < out.size(); ++i)
+    if (out[i - 1].second > out[i].first) return true;
+  // Destinations are disjoint and sorted: those a source meets are a run of them; only its own
+  // destination, lying exactly on it, may be in there.
+  for (size_t i = 0; i < src.size(); ++i) {
+    if (size[i] <= 0) continue;
+    auto first = std::upper_bound(out.begin(), out.end(), src[i],
+                                  [](int64_t v, const std::pair<int64_t, int64_t>& o) { return v < o.second; });
+    auto last = std::lower_bound(first, out.end(), src[i] + size[i],
+                                 [](const std::pair<int64_t, int64_t>& o, int64_t v) { return o.first < v; });
+    if (last - first != (src[i] == dst[i] ? 1 : 0)) return true;
+  }
+  return false;
+}
+
+// The kernels' call: norm of dense `src`, and with `dst` their scaled copies.
+Tensor clip(const std::vector<Tensor>& src, const std::vector<Tensor>* dst, float max_norm, int kind,
+            const Tensor& norm_in) {
+  const size_t n = src.size();
+  std::vector<const void*> sp(n);
+  std::vector<void*> dp(dst ? n : 0);
+  std::vector<int64_t> count(n);
+  std::vector<int32_t> type(n);
+  for (size_t i = 0; i < n; ++i) {
+    count[i] = src[i].numel();
+    type[i] = type_code(src[i]);
+    sp[i] = src[i].const_data_ptr();
+    if (dst) dp[i] = (*dst)[i].mutable_data_ptr();
+  }
+  if (dst) {
+    std::vector<int64_t> s(n), d(n), size(n);
+    for (size_t i = 0; i < n; ++i) {
+      s[i] = reinterpret_cast<int64_t>(sp[i]);
+      d[i] = reinterpret_cast<int64_t>(dp[i]);
+      size[i] = count[i] * (type[i] == LEWM_TYPE_F32 ? 4 : 2);
+    }
+    TORCH_CHECK_VALUE(!overlap(s, d, size),
+                      "gradients overlap in memory (the same one listed twice?), or an output overlaps one");
+  }
+  need_cuda(src[0]);
+  const auto opt = src[0].options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+  Tensor norm = at::empty({}, opt), ws = at::empty({LEWM_GRAD_WORKSPACE}, opt.dtype(at::kByte));
+  const int device = src[0].get_device();
+  void* stream = stream_of(src[0]);
+  float* out = static_cast<float*>(norm.mutable_data_ptr());
+  const int32_t m = static_cast<int32_t>(std::min<size_t>(n, std::numeric_limits<int32_t>::max()));
+  if (!dst) check_status(lewm_grad_norm(sp.data(), count.data(), type.data(), m, kind, mut(ws), out, device, stream));
+  else
+    check_status(lewm_grad_clip(sp.data(), dp.data(), count.data(), type.data(), m, kind, max_norm,
+                                static_cast<const float*>(ptr(norm_in)), mut(ws), out, device, stream));
+  return norm;
+}
+
+std::vector<Tensor> dense(const std::vector<Tensor>& ts) {
+  std::vector<Tensor> out;
+  out.reserve(ts.size());
+  for (const Tensor& t : ts) out.push_back(t.contiguous());  // the tensor itself where it is contiguous
+  return out;
+}
+
+// A change in place that autograd has to see.
+void bump(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor grad_norm(const std::vector<Tensor>& grads, double norm_type) {
+  at::NoGradGuard no_grad;
+  const int kind = norm_kind(norm_type);
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  check_list("grads", grads);
+  return clip(dense(grads), nullptr, 0.f, kind, Tensor());
+}
+
+std::pair<std::vector<Tensor>, Tensor> clip_grads(const std::vector<Tensor>& grads, double max_norm, double norm_type,
+                                                  const std::optional<std::vector<Tensor>>& out_given) {
+  at::NoGradGuard no_grad;
+  const int kind = norm_kind(norm_type);
+  const float limit = check_max_norm(max_norm);
+  std::vector<Tensor> out;
+  if (out_given) {
+    out = *out_given;
+    TORCH_CHECK_VALUE(out.size() == grads.size(), "out has ", out.size(), " tensors, grads ", grads.size());
+  }
+  if (grads.empty()) return {out, at::zeros({}, at::kFloat)};
+  check_list("grads", grads);
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    if (!out_given) {
+      out.push_back(at::empty(g.sizes(), g.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)));
+      continue;
+    }
+    const Tensor& o = out[i];
+    TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
+                          o.device() == g.device(),
+                      "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
+    TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");
+  }
+  Tensor norm = clip(dense(grads), &out, limit, kind, Tensor());
+  if (out_given)
+    for (const Tensor& o : out) bump(o);
+  return {std::move(out), std::move(norm)};
+}
+
+Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double norm_type, bool error_if_nonfinite) {
+  at::NoGradGuard no_grad;
+  const int kind = norm_kind(norm_type);
+  const float limit = check_max_norm(max_norm);
+  if (grads.empty()) return at::zeros({}, at::kFloat);
+  check_list("grads", grads);
+  std::vector<size_t> strided;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    if (g.is_contiguous()) continue;
+    for (int64_t d = 0; d < g.dim(); ++d)
+      TORCH_CHECK_VALUE(g.stride(d) != 0 || g.size(d) <= 1, "a gradient of shape ", g.sizes(),
+                        " shares memory between its own elements");
+    for (size_t j : strided)
+      TORCH_CHECK_VALUE(!(grads[j].const_data_ptr() == g.const_data_ptr() && grads[j].sizes() == g.sizes() &&
+                          grads[j].strides() == g.strides()),
+                        "gradients overlap in memory (the same one listed twice?)");
+    strided.push_back(i);
+  }
+  const std::vector<Tensor> ts = dense(grads);
+  Tensor norm_in;
+  if (error_if_nonfinite) {
+    norm_in = clip(ts, nullptr, 0.f, kind, Tensor());
+    TORCH_CHECK(std::isfinite(norm_in.item<float>()), "The total norm of order ", norm_type,
+                " for gradients is non-finite, so it cannot be clipped");
+  }
+  Tensor norm = clip(ts, &ts, limit, kind, norm_in);
+  for (size_t i : strided) grads[i].copy_(ts[i]);  // counts as a change by itself
+  for (const Tensor& g : grads)
+    if (g.is_contiguous()) bump(g);
+  return norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_torch_ops, m) {
+  m.attr("abi_version") = LEWM_ABI_VERSION;
+  m.def("layer_norm", torch::wrap_pybind_function(layer_norm), py::arg("x"), py::arg("weight"), py::arg("bias"),
+        py::arg("eps"));
+  m.def("ada_layer_norm", torch::wrap_pybind_function(ada_layer_norm), py::arg("x"), py::arg("shift"),
+        py::arg("scale"), py::arg("eps"));
+  m.def("grad_norm", torch::wrap_pybind_function(grad_norm), py::arg("grads"), py::arg("norm_type"));
+  m.def("clip_grads", torch::wrap_pybind_function(clip_grads), py::arg("grads"), py::arg("max_norm"),
+        py::arg("norm_type"), py::arg("out"));
+  m.def("clip_in_place", torch::wrap_pybind_function(clip_in_place), py::arg("grads"), py::arg("max_norm"),
+        py::arg("norm_type"), py::arg("error_if_nonfinite"));
+  // For tests: how a tensor's rows are read, and the overlap rule.
+  m.def("rows", [](const Tensor& t) {
+    Rows r = rows_of(t);
+    return std::make_pair(r.t, r.stride);
+  });
+  m.def("overlap", overlap);
+}
