@@ -68,7 +68,6 @@ struct NormArgs {
   int64_t rows, x_stride, dy_stride, a_stride, b_stride;
   int64_t group;       // rows per (a, b)
   int64_t items;       // groups * split
-  int64_t chunk;       // rows per item
   int split;           // items per group
   int width;
   int p_type;
@@ -92,57 +91,245 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// Two float32 values in a register pair; the packed instructions of sm_100 do both at once, each
+// rounded like the single one. The norms are bound by instructions on 16-bit rows otherwise.
+struct F2 {
+  unsigned long long u;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float v) { return f2(v, v); }
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.u));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ float both(F2 a) {
+  const float2 v = split(a);
+  return v.x + v.y;
+}
+
+// A pair of consecutive elements from and to 32 or 64 bits.
+__device__ __forceinline__ F2 unpack(const float* q) { return f2(q[0], q[1]); }
+__device__ __forceinline__ F2 unpack(const __nv_bfloat16* q) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(q);
+  return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ F2 unpack(const __half* q) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(q));
+  return f2(v.x, v.y);
+}
+__device__ __forceinline__ void pack(float* q, F2 a) {
+  const float2 v = split(a);
+  q[0] = v.x, q[1] = v.y;
+}
+__device__ __forceinline__ void pack(__nv_bfloat16* q, F2 a) {
+  const float2 v = split(a);
+  *reinterpret_cast<__nv_bfloat162*>(q) = __floats2bfloat162_rn(v.x, v.y);
+}
+__device__ __forceinline__ void pack(__half* q, F2 a) {
+  const float2 v = split(a);
+  *reinterpret_cast<__half2*>(q) = __floats2half2_rn(v.x, v.y);
+}
+
 // E consecutive elements moved as one access.
 template <typename T, int E>
 struct alignas(sizeof(T) * E) Vec {
   T v[E];
 };
 
-// E elements of type P at `q` as float32; `vec`: aligned for accesses of min(16, E sizeof(P)) bytes.
+// E elements of type P at `q` as pairs (E > 1), in accesses of min(16, E sizeof(P)) bytes if the
+// address allows it (`vec`).
 template <typename P, int E>
-__device__ __forceinline__ void load_as_float(const P* q, bool vec, float* f) {
-  if (E > 1 && vec) {
-    constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
+__device__ __forceinline__ void load_pairs(const P* q, bool vec, F2* f) {
+  constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
 #pragma unroll
-    for (int k = 0; k < E / N; ++k) {
-      const Vec<P, N> v = reinterpret_cast<const Vec<P, N>*>(q)[k];
+  for (int k = 0; k < E / N; ++k) {
+    Vec<P, N> v;
+    if (vec) {
+      v = reinterpret_cast<const Vec<P, N>*>(q)[k];
+    } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[k * N + e] = to_f(v.v[e]);
+      for (int e = 0; e < N; ++e) v.v[e] = q[k * N + e];
     }
-  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = to_f(q[e]);
+    for (int e = 0; e < N; e += 2) f[(k * N + e) / 2] = unpack(v.v + e);
   }
 }
 template <typename P, int E>
-__device__ __forceinline__ void store_from_float(P* q, bool vec, const float* f) {
-  if (E > 1 && vec) {
-    constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
+__device__ __forceinline__ void store_pairs(P* q, bool vec, const F2* f) {
+  constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
 #pragma unroll
-    for (int k = 0; k < E / N; ++k) {
-      Vec<P, N> v;
+  for (int k = 0; k < E / N; ++k) {
+    Vec<P, N> v;
 #pragma unroll
-      for (int e = 0; e < N; ++e) v.v[e] = from_f<P>(f[k * N + e]);
+    for (int e = 0; e < N; e += 2) pack(v.v + e, f[(k * N + e) / 2]);
+    if (vec) {
       reinterpret_cast<Vec<P, N>*>(q)[k] = v;
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = from_f<P>(f[e]);
+      for (int e = 0; e < N; ++e) q[k * N + e] = v.v[e];
+    }
   }
 }
-// E parameters at element offset `at`, whatever their type.
-template <int E>
-__device__ __forceinline__ void load_params(const void* p, int type, int64_t at, bool vec, float* f) {
-  if (type == LEWM_TYPE_F32) load_as_float<float, E>(static_cast<const float*>(p) + at, vec, f);
-  else if (type == LEWM_TYPE_BF16) load_as_float<__nv_bfloat16, E>(static_cast<const __nv_bfloat16*>(p) + at, vec, f);
-  else load_as_float<__half, E>(static_cast<const __half*>(p) + at, vec, f);
+// One parameter, whatever the type.
+__device__ __forceinline__ float load_param(const void* p, int type, int64_t at) {
+  if (type == LEWM_TYPE_F32) return static_cast<const float*>(p)[at];
+  if (type == LEWM_TYPE_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[at]);
+  return to_f(static_cast<const __half*>(p)[at]);
 }
-template <int E>
-__device__ __forceinline__ void store_params(void* p, int type, int64_t at, bool vec, const float* f) {
-  if (type == LEWM_TYPE_F32) store_from_float<float, E>(static_cast<float*>(p) + at, vec, f);
-  else if (type == LEWM_TYPE_BF16) store_from_float<__nv_bfloat16, E>(static_cast<__nv_bfloat16*>(p) + at, vec, f);
-  else store_from_float<__half, E>(static_cast<__half*>(p) + at, vec, f);
+__device__ __forceinline__ void store_param(void* p, int type, int64_t at, float f) {
+  if (type == LEWM_TYPE_F32) static_cast<float*>(p)[at] = f;
+  else if (type == LEWM_TYPE_BF16) static_cast<__nv_bfloat16*>(p)[at] = from_f<__nv_bfloat16>(f);
+  else static_cast<__half*>(p)[at] = from_f<__half>(f);
 }
+
+// ------------------------------------------------------------------ teams
+constexpr int block_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// What a thread holds of a row. N values as N / 2 pairs: vector i of the team's vectors lane +
+// i TPR, whose E values are pairs i E / 2 on (E > 1); or single values lane + i TPR, two of
+// consecutive i in a pair (E = 1).
+template <int E_, int NV_, int TPR_>
+struct Team {
+  static constexpr int E = E_, NV = NV_, TPR = TPR_, N = E * NV, H = N / 2;
+  static constexpr int THREADS = block_threads(TPR), TEAMS = THREADS / TPR;
+  // Vectors that lie inside every row of the tier: its narrowest row fills more than half of a
+  // team (a quarter in the tier of 65 to 256).
+  static constexpr int SURE = TPR == 8 ? 0 : N == 8 ? NV / 4 : NV / 2;
+
+  static __device__ __forceinline__ int team() { return threadIdx.x / TPR; }
+  static __device__ __forceinline__ int lane() { return threadIdx.x % TPR; }
+  // Barrier of the threads that share a row.
+  static __device__ __forceinline__ void barrier() {
+    if constexpr (TPR > 32) named_bar(1 + team(), TPR);
+    else __syncwarp();
+  }
+  // Sum over the team, the same bits in all of its threads. Teams of more than a warp add their
+  // warps' sums through `red` (a slot per warp of the block) in warp order; the caller alternates
+  // between two `red` buffers, so that one is rewritten only after a later barrier.
+  static __device__ __forceinline__ float sum(float v, float* red) {
+    constexpr int W = TPR < 32 ? TPR : 32;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TPR > 32) {
+      const int warp = threadIdx.x >> 5, w0 = team() * (TPR / 32);
+      if ((threadIdx.x & 31) == 0) red[warp] = v;
+      barrier();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) v += red[w0 + i];
+    }
+    return v;
+  }
+  static __device__ __forceinline__ float2 sum2(float2 v, float2* red) {
+    constexpr int W = TPR < 32 ? TPR : 32;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if constexpr (TPR > 32) {
+      const int warp = threadIdx.x >> 5, w0 = team() * (TPR / 32);
+      if ((threadIdx.x & 31) == 0) red[warp] = v;
+      barrier();
+      v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < TPR / 32; ++i) {
+        v.x += red[w0 + i].x;
+        v.y += red[w0 + i].y;
+      }
+    }
+    return v;
+  }
+
+  // This thread's parameters of a row of `width` at element offset `at`, `outside` beyond it.
+  static __device__ __forceinline__ void load_params(const void* p, int type, int64_t at, int width, bool vec, F2* f) {
+    if constexpr (E > 1) {
+      const int nvec = width / E;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = lane() + i * TPR;
+        if (v >= nvec) continue;
+        F2* o = f + i * (E / 2);
+        const int64_t c = at + (int64_t)v * E;
+        if (type == LEWM_TYPE_F32) load_pairs<float, E>(static_cast<const float*>(p) + c, vec, o);
+        else if (type == LEWM_TYPE_BF16) load_pairs<__nv_bfloat16, E>(static_cast<const __nv_bfloat16*>(p) + c, vec, o);
+        else load_pairs<__half, E>(static_cast<const __half*>(p) + c, vec, o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const int c = lane() + 2 * i * TPR;
+        float2 v = split(f[i]);
+        if (c < width) v.x = load_param(p, type, at + c);
+        if (c + TPR < width) v.y = load_param(p, type, at + c + TPR);
+        f[i] = f2(v.x, v.y);
+      }
+    }
+  }
+  // Stores a row of `width` values of type P at `row`.
+  template <typename P>
+  static __device__ __forceinline__ void store_row(P* row, int width, const F2* f) {
+    if constexpr (E > 1) {
+      const int nvec = width / E;
+      P* q = row + lane() * E;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i < SURE || lane() + i * TPR < nvec) store_pairs<P, E>(q + i * TPR * E, true, f + i * (E / 2));
+    } else {
+      P* q = row + lane();
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const float2 v = split(f[i]);
+        if (2 * i < SURE || lane() + 2 * i * TPR < width) q[2 * i * TPR] = from_f<P>(v.x);
+        if (2 * i + 1 < SURE || lane() + (2 * i + 1) * TPR < width) q[(2 * i + 1) * TPR] = from_f<P>(v.y);
+      }
+    }
+  }
+  static __device__ __forceinline__ void store_params(void* p, int type, int64_t at, int width, bool vec,
+                                                      const F2* f) {
+    if constexpr (E > 1) {
+      const int nvec = width / E;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int v = lane() + i * TPR;
+        if (v >= nvec) continue;
+        const F2* o = f + i * (E / 2);
+        const int64_t c = at + (int64_t)v * E;
+        if (type == LEWM_TYPE_F32) store_pairs<float, E>(static_cast<float*>(p) + c, vec, o);
+        else if (type == LEWM_TYPE_BF16) store_pairs<__nv_bfloat16, E>(static_cast<__nv_bfloat16*>(p) + c, vec, o);
+        else store_pairs<__half, E>(static_cast<__half*>(p) + c, vec, o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const int c = lane() + 2 * i * TPR;
+        const float2 v = split(f[i]);
+        if (c < width) store_param(p, type, at + c, v.x);
+        if (c + TPR < width) store_param(p, type, at + c + TPR, v.y);
+      }
+    }
+  }
+};
 
 // ------------------------------------------------------------------ ring of rows
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -161,457 +348,448 @@ __device__ __forceinline__ void cp_wait(int stages) {
   else if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else asm volatile("cp.async.wait_group 2;" ::: "memory");
 }
-template <int TPR>
-__device__ __forceinline__ void team_barrier() {
-  if constexpr (TPR > 32) __syncthreads();
-  else __syncwarp();
-}
-
-constexpr int block_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 
 // One stage of the ring for one tensor of element type P: a row of each team of the block.
 //   E > 1: vector i of a thread lies at [piece][i][thread] in 16-byte (or 8-byte) pieces; only
 //          that thread copies and reads it.
 //   E = 1: a team's row lies in its slot at its address modulo 16; any thread copies any part.
-template <typename P, int E, int NV, int TPR>
+template <typename P, typename Tm>
 struct Stage {
-  static constexpr int THREADS = block_threads(TPR), TEAMS = THREADS / TPR;
-  static constexpr int VB = E * (int)sizeof(P);           // bytes of a vector
+  static constexpr int E = Tm::E, NV = Tm::NV, TPR = Tm::TPR, THREADS = Tm::THREADS;
+  static constexpr int VB = E * (int)sizeof(P);                  // bytes of a vector
   [[maybe_unused]] static constexpr int PB = VB > 16 ? 16 : VB;  // of a piece
-  static constexpr int SLOT = NV * TPR * (int)sizeof(P) + 32;  // E = 1
-  static constexpr int BYTES = E > 1 ? NV * VB * THREADS : TEAMS * SLOT;
+  [[maybe_unused]] static constexpr int SLOT = NV * TPR * (int)sizeof(P) + 32;  // E = 1
+  static constexpr int BYTES = E > 1 ? NV * VB * THREADS : Tm::TEAMS * SLOT;
 
-  // Starts the copy of a row. [lo, hi) is the whole tensor: a 4-byte end piece of a row of 16-bit
-  // elements may take a neighbouring element along, but nothing outside the tensor.
-  static __device__ __forceinline__ void fetch(char* buf, const P* row, int width, bool live, const P* lo,
-                                               const P* hi) {
-    const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-    if (!live) return;
+  // Starts the copy of a row to the stage at `buf`. [lo, hi) is the whole tensor: a 4-byte end
+  // piece of a row of 16-bit elements may take a neighbouring element along, but nothing outside
+  // the tensor.
+  static __device__ __forceinline__ void fetch(uint32_t buf, const P* row, int width, const P* lo, const P* hi) {
+    const int lane = Tm::lane();
     if constexpr (E > 1) {
       const int nvec = width / E;
+      const char* src = reinterpret_cast<const char*>(row) + lane * VB;
+      const uint32_t dst = buf + threadIdx.x * PB;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int v = lane + i * TPR;
-        if (v >= nvec) continue;
+        if (i < Tm::SURE || lane + i * TPR < nvec) {
 #pragma unroll
-        for (int k = 0; k < VB / PB; ++k) {
-          const uint32_t dst = smem_u32(buf + ((k * NV + i) * THREADS + threadIdx.x) * PB);
-          const char* src = reinterpret_cast<const char*>(row + (int64_t)v * E) + k * PB;
-          if constexpr (PB == 16) cp_async16(dst, src);
-          else cp_async8(dst, src);
+          for (int k = 0; k < VB / PB; ++k) {
+            if constexpr (PB == 16) cp_async16(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
+            else cp_async8(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
+          }
         }
       }
     } else {
       const uintptr_t s = reinterpret_cast<uintptr_t>(row), e = s + (uintptr_t)width * sizeof(P);
-      char* slot = buf + team * SLOT;
-      const uintptr_t origin = s & ~(uintptr_t)15;  // lies at slot[0]
+      const uintptr_t origin = s & ~(uintptr_t)15;  // lies at the slot's start
+      const uint32_t slot = buf + Tm::team() * SLOT;
       const uintptr_t a0 = (s + 15) & ~(uintptr_t)15, last = e & ~(uintptr_t)15, a1 = last > a0 ? last : a0;
       for (uintptr_t a = a0 + 16 * lane; a < a1; a += 16 * TPR)
-        cp_async16(smem_u32(slot + (a - origin)), reinterpret_cast<const void*>(a));
+        cp_async16(slot + (uint32_t)(a - origin), reinterpret_cast<const void*>(a));
       if (lane < 8) {  // up to four 4-byte words before a0 and after a1
         const uintptr_t w = lane < 4 ? (s & ~(uintptr_t)3) + 4 * lane : a1 + 4 * (lane - 4);
         if (w < (lane < 4 ? (a0 < e ? a0 : e) : e)) {
           if (w >= reinterpret_cast<uintptr_t>(lo) && w + 4 <= reinterpret_cast<uintptr_t>(hi)) {
-            cp_async4(smem_u32(slot + (w - origin)), reinterpret_cast<const void*>(w));
+            cp_async4(slot + (uint32_t)(w - origin), reinterpret_cast<const void*>(w));
           } else {
             for (uintptr_t q = w; q < w + 4; q += sizeof(P))
-              if (q >= s && q < e) *reinterpret_cast<P*>(slot + (q - origin)) = *reinterpret_cast<const P*>(q);
+              if (q >= s && q < e) {
+                P* d = reinterpret_cast<P*>(__cvta_shared_to_generic(slot + (uint32_t)(q - origin)));
+                *d = *reinterpret_cast<const P*>(q);
+              }
           }
         }
       }
     }
   }
 
-  // This thread's values of a row, 0 outside it.
-  static __device__ __forceinline__ void read(const char* buf, const P* row, int width, bool live, float* f) {
-    const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  // This thread's values of a row, 0 beyond it. `row` gives the address modulo 16.
+  static __device__ __forceinline__ void read(const char* buf, const P* row, int width, F2* f) {
+    const int lane = Tm::lane();
     if constexpr (E > 1) {
       const int nvec = width / E;
+      constexpr int K = PB / (int)sizeof(P);
+      const char* src = buf + threadIdx.x * PB;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const bool in = live && lane + i * TPR < nvec;
 #pragma unroll
         for (int k = 0; k < VB / PB; ++k) {
-          constexpr int N = PB / (int)sizeof(P);
-          if (in) {
-            const Vec<P, N> v =
-                *reinterpret_cast<const Vec<P, N>*>(buf + ((k * NV + i) * THREADS + threadIdx.x) * PB);
+          F2* o = f + (i * E + k * K) / 2;
+          if (i < Tm::SURE || lane + i * TPR < nvec) {
+            const Vec<P, K> v = *reinterpret_cast<const Vec<P, K>*>(src + (k * NV + i) * THREADS * PB);
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[i * E + k * N + e] = to_f(v.v[e]);
+            for (int e = 0; e < K; e += 2) o[e / 2] = unpack(v.v + e);
           } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) f[i * E + k * N + e] = 0.f;
+            for (int e = 0; e < K; e += 2) o[e / 2] = f2(0.f);
           }
         }
       }
     } else {
-      const P* q = reinterpret_cast<const P*>(buf + team * SLOT + (reinterpret_cast<uintptr_t>(row) & 15));
+      const P* q = reinterpret_cast<const P*>(buf + Tm::team() * SLOT + (reinterpret_cast<uintptr_t>(row) & 15)) + lane;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = lane + i * TPR;
-        f[i] = live && c < width ? to_f(q[c]) : 0.f;
+      for (int i = 0; i < Tm::H; ++i) {
+        const float x = 2 * i < Tm::SURE || lane + 2 * i * TPR < width ? to_f(q[2 * i * TPR]) : 0.f;
+        const float y = 2 * i + 1 < Tm::SURE || lane + (2 * i + 1) * TPR < width ? to_f(q[(2 * i + 1) * TPR]) : 0.f;
+        f[i] = f2(x, y);
       }
     }
   }
 };
 
-// ------------------------------------------------------------------ team sums
-// Sum of `v` over the TPR threads of a team, the same bits in all of them. Teams of more than
-// a warp add their warps' sums through `red` (a slot per warp of the block) in warp order;
-// every thread of the block must call it. One barrier per call: the caller alternates between
-// two `red` buffers, so a buffer is rewritten only after a later barrier.
-template <int TPR>
-__device__ __forceinline__ float team_sum(float v, float* red) {
-  constexpr int W = TPR < 32 ? TPR : 32;
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (TPR > 32) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
-    const int w0 = warp / (TPR / 32) * (TPR / 32);
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) v += red[w0 + i];
-  }
-  return v;
-}
-template <int TPR>
-__device__ __forceinline__ float2 team_sum2(float2 v, float2* red) {
-  constexpr int W = TPR < 32 ? TPR : 32;
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  if constexpr (TPR > 32) {
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
-    __syncthreads();
-    const int w0 = warp / (TPR / 32) * (TPR / 32);
-    v = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < TPR / 32; ++i) {
-      v.x += red[w0 + i].x;
-      v.y += red[w0 + i].y;
-    }
-  }
-  return v;
-}
-
-// Rows of an item: [r0, r1) within group g.
+// Rows of an item for one team: first, first + step, ... below end, in group g. The items of a
+// group take its rows in turn, a block's worth at a time, so that the blocks sweep x in one
+// front: with a contiguous run of rows for each block DRAM gave less (73881 x 1536 float32
+// backward: 4.3 against 6.4 TB/s).
 struct Item {
-  int64_t g, r0, r1;
+  int64_t g, first, end, step;
+  int64_t iters;  // of the whole block's loop
 };
-__device__ __forceinline__ Item item_rows(const NormArgs& p, int64_t item) {
-  Item it{0, 0, 0};
-  if (item >= p.items) return it;  // no rows
-  it.g = p.split == 1 ? item : item / p.split;
-  const int64_t s = item - it.g * p.split;
-  it.r0 = it.g * p.group + s * p.chunk;
-  it.r1 = min(it.r0 + p.chunk, (it.g + 1) * p.group);
+template <int TEAMS>
+__device__ __forceinline__ Item item_rows(const NormArgs& p, int64_t base, int team) {
+  Item it{0, 0, 0, 1, p.group};
+  if (p.team_items) {
+    it.g = base + team;
+    if (it.g >= p.items) return Item{0, 0, 0, 1, p.group};  // no rows
+    it.first = it.g * p.group;
+  } else {
+    it.g = p.split == 1 ? base : base / p.split;
+    const int64_t s = base - it.g * p.split;
+    it.step = (int64_t)p.split * TEAMS;
+    it.first = it.g * p.group + s * TEAMS + team;
+    it.iters = (p.group - s * TEAMS + it.step - 1) / it.step;
+  }
+  it.end = (it.g + 1) * p.group;
   return it;
 }
 
+// A tensor's rows from the loop's first one on, advanced by pointer.
+template <typename P>
+struct Walk {
+  const P *at, *lo, *hi;
+  int64_t step;
+  __device__ __forceinline__ Walk(const void* base, int64_t rows, int64_t stride, int width, int64_t first,
+                                  int64_t step_rows)
+      : at(static_cast<const P*>(base) + first * stride),
+        lo(static_cast<const P*>(base)),
+        hi(static_cast<const P*>(base) + (rows - 1) * stride + width),
+        step(step_rows * stride) {}
+};
+
 // Blocks per SM that the registers are limited for: 80 a thread forward, 128 backward.
-constexpr int blocks_per_sm(int tpr, bool backward) { return (backward ? 512 : 768) / block_threads(tpr); }
 constexpr int bound_blocks(int tpr, bool backward) {
-  return blocks_per_sm(tpr, backward) > 0 ? blocks_per_sm(tpr, backward) : 1;
+  const int n = (backward ? 512 : 768) / block_threads(tpr);
+  return n > 0 ? n : 1;
 }
 
 // ------------------------------------------------------------------ forward
-// mu and rs of a row from the team's values (0 outside the row), which become x - mu.
-template <int N, int TPR>
-__device__ __forceinline__ float2 row_stats(float* f, const bool* in, float inv_n, float eps, float (*red)[32]) {
-  float s = 0.f, q = 0.f;
+// x - mu in place of the team's values x (0 beyond the row), mu and rs.
+template <typename Tm>
+__device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float (*red)[32]) {
+  constexpr int E = Tm::E, TPR = Tm::TPR;
+  F2 s = f2(0.f), q = f2(0.f);
 #pragma unroll
-  for (int k = 0; k < N; ++k) s += f[k];
-  const float mu = team_sum<TPR>(s, red[0]) * inv_n;
+  for (int k = 0; k < Tm::H; ++k) s = s + f[k];
+  const float mu = Tm::sum(both(s), red[0]) * inv_n;
+  const F2 nm = f2(-mu);
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    f[k] = in[k] ? f[k] - mu : 0.f;
-    q = fmaf(f[k], f[k], q);
+  for (int k = 0; k < Tm::H; ++k) {
+    f[k] = f[k] + nm;
+    if constexpr (E > 1) {
+      const int i = k / (E / 2);
+      if (i < Tm::SURE || Tm::lane() + i * TPR < width / E) q = fma2(f[k], f[k], q);
+    } else {
+      const int i = 2 * k;
+      if (i + 1 < Tm::SURE) {
+        q = fma2(f[k], f[k], q);
+      } else {
+        const float2 v = split(f[k]);
+        const F2 c = f2(Tm::lane() + i * TPR < width ? v.x : 0.f, Tm::lane() + (i + 1) * TPR < width ? v.y : 0.f);
+        q = fma2(c, c, q);
+      }
+    }
   }
-  const float var = team_sum<TPR>(q, red[1]) * inv_n;
+  const float var = Tm::sum(both(q), red[1]) * inv_n;
   return make_float2(mu, 1.0f / sqrtf(var + eps));
 }
 
-template <typename T, int E, int NV, int TPR>
-__global__ void __launch_bounds__(block_threads(TPR), bound_blocks(TPR, false)) k_norm_fwd(const NormArgs p) {
+template <typename T, typename Tm>
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_norm_fwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
-  using St = Stage<T, E, NV, TPR>;
-  constexpr int TEAMS = St::TEAMS, N = NV * E;
+  using St = Stage<T, Tm>;
+  constexpr int H = Tm::H;
   extern __shared__ __align__(16) char ring[];
   __shared__ float red[2][32];
-  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-  const int nvec = p.width / E;
   const float inv_n = 1.0f / p.width;
-  const T* x = static_cast<const T*>(p.x);
-  const T* x_end = x + (p.rows - 1) * p.x_stride + p.width;
-  bool in[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) in[k] = lane + k / E * TPR < nvec;
-  const int64_t step = p.team_items ? 1 : TEAMS;
-  const int64_t iters = (p.chunk + step - 1) / step;
-  const int64_t per_block = p.team_items ? TEAMS : 1;
+  const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * St::BYTES;
+  const int64_t per_block = p.team_items ? Tm::TEAMS : 1;
   for (int64_t base = blockIdx.x * per_block; base < p.items; base += gridDim.x * per_block) {
-    const Item it = item_rows(p, base + (p.team_items ? team : 0));
-    const int64_t first = it.r0 + (p.team_items ? 0 : team);
-    auto fetch = [&](int64_t k, int slot) {
-      const int64_t r = first + k * step;
-      St::fetch(ring + slot * St::BYTES, x + r * p.x_stride, p.width, k < iters && r < it.r1, x, x_end);
+    const Item it = item_rows<Tm::TEAMS>(p, base, Tm::team());
+    Walk<T> x(p.x, p.rows, p.x_stride, p.width, it.first, it.step);
+    const T* x_now = x.at;  // the row being computed; x.at is the one being fetched
+    int64_t left = it.first < it.end ? (it.end - it.first + it.step - 1) / it.step : 0, ahead = left;
+    uint32_t in = ring0, out = ring0;
+    auto fetch = [&]() {
+      if (ahead > 0) St::fetch(in, x.at, p.width, x.lo, x.hi);
+      --ahead;
+      x.at += x.step;
+      in = in + St::BYTES == ring_end ? ring0 : in + St::BYTES;
       cp_commit();
     };
-    for (int k = 0; k < p.stages - 1; ++k) fetch(k, k);
-    float ga[N], gb[N];
+    for (int k = 0; k < p.stages - 1; ++k) fetch();
+    F2 ga[H], gb[H];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * TPR;
-#pragma unroll
-      for (int e = 0; e < E; ++e) ga[i * E + e] = 1.f, gb[i * E + e] = 0.f;
-      if (v < nvec && it.r0 < it.r1) {
-        if (p.a) load_params<E>(p.a, p.p_type, it.g * p.a_stride + (int64_t)v * E, p.p_vec, ga + i * E);
-        if (p.b) load_params<E>(p.b, p.p_type, it.g * p.b_stride + (int64_t)v * E, p.p_vec, gb + i * E);
-        if (p.one_plus) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) ga[i * E + e] += 1.f;
-        }
-      }
+    for (int k = 0; k < H; ++k) ga[k] = f2(p.one_plus ? 0.f : 1.f), gb[k] = f2(0.f);
+    if (left > 0) {
+      if (p.a) Tm::load_params(p.a, p.p_type, it.g * p.a_stride, p.width, p.p_vec, ga);
+      if (p.b) Tm::load_params(p.b, p.p_type, it.g * p.b_stride, p.width, p.p_vec, gb);
     }
-    int slot = 0;
-    for (int64_t k = 0; k < iters; ++k) {
-      const int64_t r = first + k * step;
-      const bool live = r < it.r1;
+    if (p.one_plus) {
+#pragma unroll
+      for (int k = 0; k < H; ++k) ga[k] = ga[k] + f2(1.f);
+    }
+    int64_t r = it.first;
+    T* y = static_cast<T*>(p.out) + r * p.width;
+    for (int64_t k = 0; k < it.iters; ++k) {
       cp_wait(p.stages);
-      if constexpr (E == 1) team_barrier<TPR>();
-      fetch(k + p.stages - 1, slot == 0 ? p.stages - 1 : slot - 1);
-      float f[N];
-      St::read(ring + slot * St::BYTES, x + r * p.x_stride, p.width, live, f);
-      if (++slot == p.stages) slot = 0;
-      const float2 ms = row_stats<N, TPR>(f, in, inv_n, p.eps, red);
-      if (!live) continue;
-      if (p.stats && lane == 0) {
-        p.stats[r] = ms.x;
-        p.stats[p.rows + r] = ms.y;
-      }
-      T* y = static_cast<T*>(p.out) + r * p.width;
+      if constexpr (Tm::E == 1) Tm::barrier();
+      fetch();
+      F2 f[H];
+      if (left > 0) {
+        St::read(ring + (out - ring0), x_now, p.width, f);
+      } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = lane + i * TPR;
-        if (v >= nvec) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[i * E + e] = fmaf(f[i * E + e] * ms.y, ga[i * E + e], gb[i * E + e]);
-        store_from_float<T, E>(y + (int64_t)v * E, true, f + i * E);
+        for (int h = 0; h < H; ++h) f[h] = f2(0.f);
       }
+      out = out + St::BYTES == ring_end ? ring0 : out + St::BYTES;
+      const float2 ms = row_stats<Tm>(f, p.width, inv_n, p.eps, red);
+      if (left > 0) {
+        if (p.stats && Tm::lane() == 0) {
+          p.stats[r] = ms.x;
+          p.stats[p.rows + r] = ms.y;
+        }
+        const F2 rs = f2(ms.y);
+#pragma unroll
+        for (int h = 0; h < H; ++h) f[h] = fma2(f[h] * rs, ga[h], gb[h]);
+        Tm::store_row(y, p.width, f);
+      }
+      --left;
+      r += it.step;
+      y += it.step * p.width;
+      x_now += x.step;
     }
-    if constexpr (E == 1) team_barrier<TPR>();  // the ring is refilled for the next item
+    if constexpr (Tm::E == 1) Tm::barrier();  // the ring is refilled for the next item
   }
 }
 
 // A modulation row per row of x: rows in a grid stride, scale and shift in the ring beside x.
-template <typename T, typename P, int E, int NV, int TPR>
-__global__ void __launch_bounds__(block_threads(TPR), bound_blocks(TPR, false)) k_rowmod_fwd(const NormArgs p) {
+template <typename T, typename P, typename Tm>
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_rowmod_fwd(const NormArgs p) {
   griddep_wait();
-  using St = Stage<T, E, NV, TPR>;
-  using Sp = Stage<P, E, NV, TPR>;
-  constexpr int TEAMS = St::TEAMS, N = NV * E, BYTES = St::BYTES + 2 * Sp::BYTES;
+  using St = Stage<T, Tm>;
+  using Sp = Stage<P, Tm>;
+  constexpr int H = Tm::H, BYTES = St::BYTES + 2 * Sp::BYTES;
   extern __shared__ __align__(16) char ring[];
   __shared__ float red[2][32];
-  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-  const int nvec = p.width / E;
   const float inv_n = 1.0f / p.width;
-  const T* x = static_cast<const T*>(p.x);
-  const P* a = static_cast<const P*>(p.a);
-  const P* b = static_cast<const P*>(p.b);
-  const T* x_end = x + (p.rows - 1) * p.x_stride + p.width;
-  const P* a_end = a + (p.rows - 1) * p.a_stride + p.width;
-  const P* b_end = b + (p.rows - 1) * p.b_stride + p.width;
-  bool in[N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) in[k] = lane + k / E * TPR < nvec;
-  const int64_t first = (int64_t)blockIdx.x * TEAMS + team, step = (int64_t)gridDim.x * TEAMS;
-  const int64_t iters = (p.rows - (int64_t)blockIdx.x * TEAMS + step - 1) / step;
-  auto fetch = [&](int64_t k, int slot) {
-    const int64_t r = first + k * step;
-    const bool live = r < p.rows;
-    char* buf = ring + slot * BYTES;
-    St::fetch(buf, x + r * p.x_stride, p.width, live, x, x_end);
-    Sp::fetch(buf + St::BYTES, a + r * p.a_stride, p.width, live, a, a_end);
-    Sp::fetch(buf + St::BYTES + Sp::BYTES, b + r * p.b_stride, p.width, live, b, b_end);
+  const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
+  const int64_t first = (int64_t)blockIdx.x * Tm::TEAMS + Tm::team(), step = (int64_t)gridDim.x * Tm::TEAMS;
+  const int64_t iters = (p.rows - (int64_t)blockIdx.x * Tm::TEAMS + step - 1) / step;
+  Walk<T> x(p.x, p.rows, p.x_stride, p.width, first, step);
+  Walk<P> a(p.a, p.rows, p.a_stride, p.width, first, step), b(p.b, p.rows, p.b_stride, p.width, first, step);
+  const T* x_now = x.at;
+  const P *a_now = a.at, *b_now = b.at;
+  int64_t left = first < p.rows ? (p.rows - first + step - 1) / step : 0, ahead = left;
+  uint32_t in = ring0, out = ring0;
+  auto fetch = [&]() {
+    if (ahead > 0) {
+      St::fetch(in, x.at, p.width, x.lo, x.hi);
+      Sp::fetch(in + St::BYTES, a.at, p.width, a.lo, a.hi);
+      Sp::fetch(in + St::BYTES + Sp::BYTES, b.at, p.width, b.lo, b.hi);
+    }
+    --ahead;
+    x.at += x.step, a.at += a.step, b.at += b.step;
+    in = in + BYTES == ring_end ? ring0 : in + BYTES;
     cp_commit();
   };
-  for (int k = 0; k < p.stages - 1; ++k) fetch(k, k);
-  int slot = 0;
+  for (int k = 0; k < p.stages - 1; ++k) fetch();
+  int64_t r = first;
+  T* y = static_cast<T*>(p.out) + r * p.width;
   for (int64_t k = 0; k < iters; ++k) {
-    const int64_t r = first + k * step;
-    const bool live = r < p.rows;
     cp_wait(p.stages);
-    if constexpr (E == 1) team_barrier<TPR>();
-    fetch(k + p.stages - 1, slot == 0 ? p.stages - 1 : slot - 1);
-    const char* buf = ring + slot * BYTES;
-    float f[N];
-    St::read(buf, x + r * p.x_stride, p.width, live, f);
-    const float2 ms = row_stats<N, TPR>(f, in, inv_n, p.eps, red);
-    float ga[N], gb[N];
-    Sp::read(buf + St::BYTES, a + r * p.a_stride, p.width, live, ga);
-    Sp::read(buf + St::BYTES + Sp::BYTES, b + r * p.b_stride, p.width, live, gb);
-    if (++slot == p.stages) slot = 0;
-    if (!live) continue;
-    if (p.stats && lane == 0) {
-      p.stats[r] = ms.x;
-      p.stats[p.rows + r] = ms.y;
-    }
-    T* y = static_cast<T*>(p.out) + r * p.width;
+    if constexpr (Tm::E == 1) Tm::barrier();
+    fetch();
+    const char* buf = ring + (out - ring0);
+    out = out + BYTES == ring_end ? ring0 : out + BYTES;
+    F2 f[H];
+    if (left > 0) {
+      St::read(buf, x_now, p.width, f);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * TPR;
-      if (v >= nvec) continue;
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[i * E + e] = fmaf(f[i * E + e] * ms.y, 1.f + ga[i * E + e], gb[i * E + e]);
-      store_from_float<T, E>(y + (int64_t)v * E, true, f + i * E);
+      for (int h = 0; h < H; ++h) f[h] = f2(0.f);
     }
+    const float2 ms = row_stats<Tm>(f, p.width, inv_n, p.eps, red);
+    if (left > 0) {
+      if (p.stats && Tm::lane() == 0) {
+        p.stats[r] = ms.x;
+        p.stats[p.rows + r] = ms.y;
+      }
+      F2 ga[H], gb[H];
+      Sp::read(buf + St::BYTES, a_now, p.width, ga);
+      Sp::read(buf + St::BYTES + Sp::BYTES, b_now, p.width, gb);
+      const F2 rs = f2(ms.y), one = f2(1.f);
+#pragma unroll
+      for (int h = 0; h < H; ++h) f[h] = fma2(f[h] * rs, ga[h] + one, gb[h]);
+      Tm::store_row(y, p.width, f);
+    }
+    --left;
+    r += step;
+    y += step * p.width;
+    x_now += x.step, a_now += a.step, b_now += b.step;
   }
 }
 
 // ------------------------------------------------------------------ backward
-// Where the sums of E columns from `col` on of an item go. Partial sums are float4-aligned where
-// E > 1 (the width is then a multiple of 4).
-template <int E>
-__device__ __forceinline__ void store_sums(const NormArgs& p, int64_t item, int64_t g, int64_t col, bool vec,
-                                           const float* a, const float* b) {
-  if (p.split > 1) {
-    float* w = p.ws + item * 2 * p.width + col;
-    store_from_float<float, E>(w, true, a);
-    store_from_float<float, E>(w + p.width, true, b);
-  } else {
-    if (p.da) store_params<E>(p.da, p.p_type, g * p.width + col, vec, a);
-    if (p.db) store_params<E>(p.db, p.p_type, g * p.width + col, vec, b);
-  }
+// dx of a row from z, d and the row's sums.
+template <typename T, typename Tm>
+__device__ __forceinline__ void store_dx(T* dx, int width, const F2* z, F2* d, float2 s, float inv_n, float rs) {
+  const F2 m1 = f2(-s.x * inv_n), m2 = f2(-s.y * inv_n), r = f2(rs);
+#pragma unroll
+  for (int h = 0; h < Tm::H; ++h) d[h] = fma2(z[h], m2, d[h] + m1) * r;
+  Tm::store_row(dx, width, d);
 }
 
-template <typename T, int E, int NV, int TPR>
-__global__ void __launch_bounds__(block_threads(TPR), bound_blocks(TPR, true)) k_norm_bwd(const NormArgs p) {
+template <typename T, typename Tm>
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_norm_bwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
-  using St = Stage<T, E, NV, TPR>;
-  constexpr int THREADS = St::THREADS, TEAMS = St::TEAMS, N = NV * E, BYTES = 2 * St::BYTES;
+  // The whole grid is resident by now, so the reduction's blocks take no slot from it; they
+  // wait for its end with their launch behind them.
+  if (p.split > 1) griddep_launch();
+  using St = Stage<T, Tm>;
+  constexpr int THREADS = Tm::THREADS, TEAMS = Tm::TEAMS, TPR = Tm::TPR, E = Tm::E, H = Tm::H, BYTES = 2 * St::BYTES;
   extern __shared__ __align__(16) char ring[];
   __shared__ float2 red[2][32];
   // The teams' sums of a slab of columns; the ring (two stages at least) is idle then.
   float2* sums = reinterpret_cast<float2*>(ring);
-  static_assert(TEAMS == 1 || TEAMS * TPR * E * (int)sizeof(float2) <= 2 * BYTES, "sums fit the ring");
-  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-  const int nvec = p.width / E;
+  constexpr int SLAB = TPR * (E > 1 ? E : 2);  // columns added up at a time
+  static_assert(TEAMS == 1 || TEAMS * SLAB * (int)sizeof(float2) <= 2 * BYTES, "sums fit the ring");
   const float inv_n = 1.0f / p.width;
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  const T* x_end = x + (p.rows - 1) * p.x_stride + p.width;
-  const T* dy_end = dy + (p.rows - 1) * p.dy_stride + p.width;
-  const int64_t step = p.team_items ? 1 : TEAMS;
-  const int64_t iters = (p.chunk + step - 1) / step;
+  const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
   const int64_t per_block = p.team_items ? TEAMS : 1;
   int flip = 0;
   for (int64_t base = blockIdx.x * per_block; base < p.items; base += gridDim.x * per_block) {
-    const int64_t item = base + (p.team_items ? team : 0);
-    const Item it = item_rows(p, item);
-    const int64_t first = it.r0 + (p.team_items ? 0 : team);
-    auto fetch = [&](int64_t k, int slot) {
-      const int64_t r = first + k * step;
-      const bool live = k < iters && r < it.r1;
-      char* buf = ring + slot * BYTES;
-      St::fetch(buf, x + r * p.x_stride, p.width, live, x, x_end);
-      St::fetch(buf + St::BYTES, dy + r * p.dy_stride, p.width, live, dy, dy_end);
+    const Item it = item_rows<TEAMS>(p, base, Tm::team());
+    Walk<T> x(p.x, p.rows, p.x_stride, p.width, it.first, it.step);
+    Walk<T> dy(p.dy, p.rows, p.dy_stride, p.width, it.first, it.step);
+    const T *x_now = x.at, *dy_now = dy.at;
+    int64_t left = it.first < it.end ? (it.end - it.first + it.step - 1) / it.step : 0, ahead = left;
+    const bool any = left > 0;
+    uint32_t in = ring0, out = ring0;
+    auto fetch = [&]() {
+      if (ahead > 0) {
+        St::fetch(in, x.at, p.width, x.lo, x.hi);
+        St::fetch(in + St::BYTES, dy.at, p.width, dy.lo, dy.hi);
+      }
+      --ahead;
+      x.at += x.step, dy.at += dy.step;
+      in = in + BYTES == ring_end ? ring0 : in + BYTES;
       cp_commit();
     };
-    for (int k = 0; k < p.stages - 1; ++k) fetch(k, k);
-    float ga[N], sa[N], sb[N];
+    for (int k = 0; k < p.stages - 1; ++k) fetch();
+    F2 ga[H], sa[H], sb[H];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * TPR;
+    for (int k = 0; k < H; ++k) ga[k] = f2(p.one_plus ? 0.f : 1.f), sa[k] = sb[k] = f2(0.f);
+    if (p.a && any) Tm::load_params(p.a, p.p_type, it.g * p.a_stride, p.width, p.p_vec, ga);
+    if (p.one_plus) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) ga[i * E + e] = 1.f, sa[i * E + e] = 0.f, sb[i * E + e] = 0.f;
-      if (p.a && v < nvec && it.r0 < it.r1) {
-        load_params<E>(p.a, p.p_type, it.g * p.a_stride + (int64_t)v * E, p.p_vec, ga + i * E);
-        if (p.one_plus) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) ga[i * E + e] += 1.f;
-        }
-      }
+      for (int k = 0; k < H; ++k) ga[k] = ga[k] + f2(1.f);
     }
     // Statistics of the first row; each row loads the next one's.
+    const float* stat = p.stats + it.first;
     float mu = 0.f, rs = 0.f;
-    if (first < it.r1) mu = p.stats[first], rs = p.stats[p.rows + first];
-    int slot = 0;
-    for (int64_t k = 0; k < iters; ++k) {
-      const int64_t r = first + k * step;
-      const bool live = r < it.r1;
+    if (any) mu = stat[0], rs = stat[p.rows];
+    T* dx = static_cast<T*>(p.out) + it.first * p.width;
+    for (int64_t k = 0; k < it.iters; ++k) {
       cp_wait(p.stages);
-      if constexpr (E == 1) team_barrier<TPR>();
-      fetch(k + p.stages - 1, slot == 0 ? p.stages - 1 : slot - 1);
+      if constexpr (E == 1) Tm::barrier();
+      fetch();
+      stat += it.step;
       float mu_next = 0.f, rs_next = 0.f;
-      if (r + step < it.r1) mu_next = p.stats[r + step], rs_next = p.stats[p.rows + r + step];
-      const char* buf = ring + slot * BYTES;
-      if (++slot == p.stages) slot = 0;
-      float z[N], g[N];
-      St::read(buf, x + r * p.x_stride, p.width, live, z);
-      St::read(buf + St::BYTES, dy + r * p.dy_stride, p.width, live, g);
+      if (left > 1) mu_next = stat[0], rs_next = stat[p.rows];
+      const char* buf = ring + (out - ring0);
+      out = out + BYTES == ring_end ? ring0 : out + BYTES;
+      F2 z[H], d[H];
       float2 s = make_float2(0.f, 0.f);
+      if (left > 0) {
+        St::read(buf, x_now, p.width, z);
+        St::read(buf + St::BYTES, dy_now, p.width, d);
+        const F2 nm = f2(-mu), r = f2(rs);
+        F2 s1 = f2(0.f), s2 = f2(0.f);
+        // Beyond the row dy is 0 and adds nothing.
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        // Values outside the row are 0 and leave every sum as it is, but for a row whose
-        // statistics are not finite: 0 times infinity would reach the other columns' sums.
-        if (!(live && lane + i * TPR < nvec)) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int c = i * E + e;
-          z[c] = (z[c] - mu) * rs;
-          sa[c] = fmaf(g[c], z[c], sa[c]);
-          sb[c] += g[c];
-          g[c] *= ga[c];
-          s.x += g[c];
-          s.y = fmaf(g[c], z[c], s.y);
+        for (int h = 0; h < H; ++h) {
+          z[h] = (z[h] + nm) * r;
+          sa[h] = fma2(d[h], z[h], sa[h]);
+          sb[h] = sb[h] + d[h];
+          d[h] = d[h] * ga[h];
+          s1 = s1 + d[h];
+          s2 = fma2(d[h], z[h], s2);
         }
+        s = make_float2(both(s1), both(s2));
       }
       if (p.out) {
-        s = team_sum2<TPR>(s, red[flip]);
+        s = Tm::sum2(s, red[flip]);
         flip ^= 1;
-        const float m1 = s.x * inv_n, m2 = s.y * inv_n;
-        T* o = static_cast<T*>(p.out) + r * p.width;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int v = lane + i * TPR;
-          if (!live || v >= nvec) continue;
-#pragma unroll
-          for (int e = 0; e < E; ++e) g[i * E + e] = rs * (g[i * E + e] - m1 - z[i * E + e] * m2);
-          store_from_float<T, E>(o + (int64_t)v * E, true, g + i * E);
-        }
+        if (left > 0) store_dx<T, Tm>(dx, p.width, z, d, s, inv_n, rs);
       }
+      --left;
       mu = mu_next;
       rs = rs_next;
+      dx += it.step * p.width;
+      x_now += x.step, dy_now += dy.step;
     }
-    if constexpr (E == 1) team_barrier<TPR>();  // the ring is refilled for the next item
+    if constexpr (E == 1) Tm::barrier();  // the ring is refilled for the next item
     if (!p.da && !p.db) continue;
     if (p.team_items || TEAMS == 1) {
-      if (it.r0 >= it.r1) continue;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = lane + i * TPR;
-        if (v < nvec) store_sums<E>(p, item, it.g, (int64_t)v * E, p.p_vec, sa + i * E, sb + i * E);
+      if (!any) continue;
+      if (p.split > 1) {  // rows of partial sums are 16-byte aligned where E > 1
+        float* w = p.ws + base * 2 * p.width;
+        Tm::store_params(w, LEWM_TYPE_F32, 0, p.width, true, sa);
+        Tm::store_params(w, LEWM_TYPE_F32, p.width, p.width, true, sb);
+      } else {
+        if (p.da) Tm::store_params(p.da, p.p_type, it.g * p.width, p.width, p.p_vec, sa);
+        if (p.db) Tm::store_params(p.db, p.p_type, it.g * p.width, p.width, p.p_vec, sb);
       }
     } else {
-      // Add the teams' sums in team order, a slab of TPR vectors of columns at a time.
+      // Add the teams' sums in team order, a slab of columns at a time.
+      constexpr int PAIRS = E > 1 ? E / 2 : 1;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (i * TPR >= nvec) break;
+      for (int i = 0; i < H / PAIRS; ++i) {
+        if (i * SLAB >= p.width) break;
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E; ++e) sums[team * TPR * E + lane * E + e] = make_float2(sa[i * E + e], sb[i * E + e]);
+        for (int k = 0; k < PAIRS; ++k) {
+          const float2 a = split(sa[i * PAIRS + k]), b = split(sb[i * PAIRS + k]);
+          const int c = E > 1 ? Tm::lane() * E + 2 * k : Tm::lane(), next = E > 1 ? c + 1 : c + TPR;
+          sums[Tm::team() * SLAB + c] = make_float2(a.x, b.x);
+          sums[Tm::team() * SLAB + next] = make_float2(a.y, b.y);
+        }
         __syncthreads();
-        for (int c = threadIdx.x; c < TPR * E; c += THREADS) {
+        for (int c = threadIdx.x; c < SLAB; c += THREADS) {
+          const int64_t col = (int64_t)i * SLAB + c;
+          if (col >= p.width) continue;
           float a = 0.f, b = 0.f;
 #pragma unroll
-          for (int t = 0; t < TEAMS; ++t) a += sums[t * TPR * E + c].x, b += sums[t * TPR * E + c].y;
-          const int64_t col = (int64_t)i * TPR * E + c;
-          if (col < p.width) store_sums<1>(p, item, it.g, col, false, &a, &b);
+          for (int t = 0; t < TEAMS; ++t) a += sums[t * SLAB + c].x, b += sums[t * SLAB + c].y;
+          if (p.split > 1) {
+            float* w = p.ws + base * 2 * p.width + col;
+            w[0] = a;
+            w[p.width] = b;
+          } else {
+            if (p.da) store_param(p.da, p.p_type, it.g * p.width + col, a);
+            if (p.db) store_param(p.db, p.p_type, it.g * p.width + col, b);
+          }
         }
       }
       __syncthreads();
@@ -620,96 +798,97 @@ __global__ void __launch_bounds__(block_threads(TPR), bound_blocks(TPR, true)) k
 }
 
 // A modulation row per row of x: d scale = dy z and d shift = dy row by row, nothing to sum up.
-template <typename T, typename P, int E, int NV, int TPR>
-__global__ void __launch_bounds__(block_threads(TPR), bound_blocks(TPR, false)) k_rowmod_bwd(const NormArgs p) {
+template <typename T, typename P, typename Tm>
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_rowmod_bwd(const NormArgs p) {
   griddep_wait();
-  using St = Stage<T, E, NV, TPR>;
-  using Sp = Stage<P, E, NV, TPR>;
-  constexpr int TEAMS = St::TEAMS, N = NV * E, BYTES = 2 * St::BYTES + Sp::BYTES;
+  using St = Stage<T, Tm>;
+  using Sp = Stage<P, Tm>;
+  constexpr int H = Tm::H, BYTES = 2 * St::BYTES + Sp::BYTES;
   extern __shared__ __align__(16) char ring[];
   __shared__ float2 red[2][32];
-  const int team = threadIdx.x / TPR, lane = threadIdx.x % TPR;
-  const int nvec = p.width / E;
   const float inv_n = 1.0f / p.width;
-  const T* x = static_cast<const T*>(p.x);
-  const T* dy = static_cast<const T*>(p.dy);
-  const P* a = static_cast<const P*>(p.a);
-  const T* x_end = x + (p.rows - 1) * p.x_stride + p.width;
-  const T* dy_end = dy + (p.rows - 1) * p.dy_stride + p.width;
-  const P* a_end = a + (p.rows - 1) * p.a_stride + p.width;
-  const int64_t first = (int64_t)blockIdx.x * TEAMS + team, step = (int64_t)gridDim.x * TEAMS;
-  const int64_t iters = (p.rows - (int64_t)blockIdx.x * TEAMS + step - 1) / step;
-  int flip = 0;
-  auto fetch = [&](int64_t k, int slot) {
-    const int64_t r = first + k * step;
-    const bool live = r < p.rows;
-    char* buf = ring + slot * BYTES;
-    St::fetch(buf, x + r * p.x_stride, p.width, live, x, x_end);
-    St::fetch(buf + St::BYTES, dy + r * p.dy_stride, p.width, live, dy, dy_end);
-    Sp::fetch(buf + 2 * St::BYTES, a + r * p.a_stride, p.width, live, a, a_end);
+  const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
+  const int64_t first = (int64_t)blockIdx.x * Tm::TEAMS + Tm::team(), step = (int64_t)gridDim.x * Tm::TEAMS;
+  const int64_t iters = (p.rows - (int64_t)blockIdx.x * Tm::TEAMS + step - 1) / step;
+  Walk<T> x(p.x, p.rows, p.x_stride, p.width, first, step), dy(p.dy, p.rows, p.dy_stride, p.width, first, step);
+  Walk<P> a(p.a, p.rows, p.a_stride, p.width, first, step);
+  const T *x_now = x.at, *dy_now = dy.at;
+  const P* a_now = a.at;
+  int64_t left = first < p.rows ? (p.rows - first + step - 1) / step : 0, ahead = left;
+  uint32_t in = ring0, out = ring0;
+  auto fetch = [&]() {
+    if (ahead > 0) {
+      St::fetch(in, x.at, p.width, x.lo, x.hi);
+      St::fetch(in + St::BYTES, dy.at, p.width, dy.lo, dy.hi);
+      Sp::fetch(in + 2 * St::BYTES, a.at, p.width, a.lo, a.hi);
+    }
+    --ahead;
+    x.at += x.step, dy.at += dy.step, a.at += a.step;
+    in = in + BYTES == ring_end ? ring0 : in + BYTES;
     cp_commit();
   };
-  for (int k = 0; k < p.stages - 1; ++k) fetch(k, k);
+  for (int k = 0; k < p.stages - 1; ++k) fetch();
+  const float* stat = p.stats + first;
   float mu = 0.f, rs = 0.f;
-  if (first < p.rows) mu = p.stats[first], rs = p.stats[p.rows + first];
-  int slot = 0;
+  if (left > 0) mu = stat[0], rs = stat[p.rows];
+  int64_t at = first * p.width;
+  int flip = 0;
   for (int64_t k = 0; k < iters; ++k) {
-    const int64_t r = first + k * step;
-    const bool live = r < p.rows;
     cp_wait(p.stages);
-    if constexpr (E == 1) team_barrier<TPR>();
-    fetch(k + p.stages - 1, slot == 0 ? p.stages - 1 : slot - 1);
+    if constexpr (Tm::E == 1) Tm::barrier();
+    fetch();
+    stat += step;
     float mu_next = 0.f, rs_next = 0.f;
-    if (r + step < p.rows) mu_next = p.stats[r + step], rs_next = p.stats[p.rows + r + step];
-    const char* buf = ring + slot * BYTES;
-    if (++slot == p.stages) slot = 0;
-    float z[N], g[N], ga[N];
-    St::read(buf, x + r * p.x_stride, p.width, live, z);
-    St::read(buf + St::BYTES, dy + r * p.dy_stride, p.width, live, g);
-    Sp::read(buf + 2 * St::BYTES, a + r * p.a_stride, p.width, live, ga);
+    if (left > 1) mu_next = stat[0], rs_next = stat[p.rows];
+    const char* buf = ring + (out - ring0);
+    out = out + BYTES == ring_end ? ring0 : out + BYTES;
+    F2 z[H], d[H];
     float2 s = make_float2(0.f, 0.f);
+    if (left > 0) {
+      F2 t[H];
+      St::read(buf, x_now, p.width, z);
+      St::read(buf + St::BYTES, dy_now, p.width, d);
+      if (p.db) Tm::store_row(static_cast<P*>(p.db) + at, p.width, d);
+      const F2 nm = f2(-mu), r = f2(rs), one = f2(1.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = lane + i * TPR;
-      if (!live || v >= nvec) continue;
-      if (p.db) store_from_float<P, E>(static_cast<P*>(p.db) + r * p.width + (int64_t)v * E, true, g + i * E);
-      float dz[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = i * E + e;
-        z[c] = (z[c] - mu) * rs;
-        dz[e] = g[c] * z[c];
-        g[c] *= 1.f + ga[c];
-        s.x += g[c];
-        s.y = fmaf(g[c], z[c], s.y);
+      for (int h = 0; h < H; ++h) {
+        z[h] = (z[h] + nm) * r;
+        t[h] = d[h] * z[h];
       }
-      if (p.da) store_from_float<P, E>(static_cast<P*>(p.da) + r * p.width + (int64_t)v * E, true, dz);
+      if (p.da) Tm::store_row(static_cast<P*>(p.da) + at, p.width, t);
+      Sp::read(buf + 2 * St::BYTES, a_now, p.width, t);
+      F2 s1 = f2(0.f), s2 = f2(0.f);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        d[h] = d[h] * (t[h] + one);
+        s1 = s1 + d[h];
+        s2 = fma2(d[h], z[h], s2);
+      }
+      s = make_float2(both(s1), both(s2));
     }
     if (p.out) {
-      s = team_sum2<TPR>(s, red[flip]);
+      s = Tm::sum2(s, red[flip]);
       flip ^= 1;
-      const float m1 = s.x * inv_n, m2 = s.y * inv_n;
-      T* o = static_cast<T*>(p.out) + r * p.width;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = lane + i * TPR;
-        if (!live || v >= nvec) continue;
-#pragma unroll
-        for (int e = 0; e < E; ++e) g[i * E + e] = rs * (g[i * E + e] - m1 - z[i * E + e] * m2);
-        store_from_float<T, E>(o + (int64_t)v * E, true, g + i * E);
-      }
+      if (left > 0) store_dx<T, Tm>(static_cast<T*>(p.out) + at, p.width, z, d, s, inv_n, rs);
     }
+    --left;
     mu = mu_next;
     rs = rs_next;
+    at += step * p.width;
+    x_now += x.step, dy_now += dy.step, a_now += a.step;
   }
 }
 
-// Sum of the `split` partial sums of each group, in item order within 32 interleaved runs and
-// then over the runs: 32 columns x 32 rows per block, grid (column tiles, groups, a or b).
-__global__ void __launch_bounds__(1024) k_norm_reduce(const NormArgs p) {
+// Sum of the `split` partial sums of each group in a fixed order: R interleaved runs of items, then
+// the runs. 32 columns x R runs per block, grid (column tiles, groups, a or b); with R = 1 a
+// thread adds a column's few partials by itself and 8 column tiles share a block.
+template <int R>
+__global__ void __launch_bounds__(R > 1 ? 32 * R : 256) k_norm_reduce(const NormArgs p) {
   griddep_wait();
-  __shared__ float part[32][33];
-  const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  __shared__ float part[R][33];
+  constexpr int COLS = R > 1 ? 32 : 256;
+  const int cx = R > 1 ? threadIdx.x % 32 : threadIdx.x, run = R > 1 ? threadIdx.x / 32 : 0;
+  const int64_t col = (int64_t)blockIdx.x * COLS + cx;
   void* out = blockIdx.z ? p.db : p.da;
   if (!out) return;
   const int64_t groups = p.items / p.split;
@@ -717,21 +896,28 @@ __global__ void __launch_bounds__(1024) k_norm_reduce(const NormArgs p) {
     float s = 0.f;
     if (col < p.width) {
       const float* w = p.ws + (g * p.split * 2 + blockIdx.z) * p.width + col;
-#pragma unroll 4
-      for (int i = threadIdx.y; i < p.split; i += 32) s += w[(int64_t)i * 2 * p.width];
+#pragma unroll 8
+      for (int i = run; i < p.split; i += R) s += w[(int64_t)i * 2 * p.width];
     }
-    part[threadIdx.y][threadIdx.x] = s;
-    __syncthreads();
-    // Warp c adds column c's 32 runs.
-    float t = warp_sum(part[threadIdx.x][threadIdx.y]);
-    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && c < p.width) store_params<1>(out, p.p_type, g * p.width + c, false, &t);
-    __syncthreads();
+    if constexpr (R == 1) {
+      if (col < p.width) store_param(out, p.p_type, g * p.width + col, s);
+    } else {
+      part[run][cx] = s;
+      __syncthreads();
+      if (run == 0 && col < p.width) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) t += part[i][cx];
+        store_param(out, p.p_type, g * p.width + col, t);
+      }
+      __syncthreads();
+    }
   }
 }
 
 // ------------------------------------------------------------------ rows of more than kMaxRowBytes
 // One block per row, the row re-read from L2 for each pass.
+using Wide = Team<1, 2, 1024>;
 template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
   griddep_wait();
@@ -741,12 +927,12 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
     const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
     float s = 0.f, q = 0.f;
     for (int c = threadIdx.x; c < p.width; c += 1024) s += to_f(x[c]);
-    const float mu = team_sum<1024>(s, red[0]) * inv_n;
+    const float mu = Wide::sum(s, red[0]) * inv_n;
     for (int c = threadIdx.x; c < p.width; c += 1024) {
       const float d = to_f(x[c]) - mu;
       q = fmaf(d, d, q);
     }
-    const float rs = 1.0f / sqrtf(team_sum<1024>(q, red[1]) * inv_n + p.eps);
+    const float rs = 1.0f / sqrtf(Wide::sum(q, red[1]) * inv_n + p.eps);
     if (p.stats && threadIdx.x == 0) {
       p.stats[r] = mu;
       p.stats[p.rows + r] = rs;
@@ -755,8 +941,8 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
     T* y = static_cast<T*>(p.out) + r * p.width;
     for (int c = threadIdx.x; c < p.width; c += 1024) {
       float a = 1.f, b = 0.f;
-      if (p.a) load_params<1>(p.a, p.p_type, g * p.a_stride + c, false, &a);
-      if (p.b) load_params<1>(p.b, p.p_type, g * p.b_stride + c, false, &b);
+      if (p.a) a = load_param(p.a, p.p_type, g * p.a_stride + c);
+      if (p.b) b = load_param(p.b, p.p_type, g * p.b_stride + c);
       if (p.one_plus) a += 1.f;
       y[c] = from_f<T>(fmaf((to_f(x[c]) - mu) * rs, a, b));
     }
@@ -776,7 +962,7 @@ __global__ void __launch_bounds__(1024) k_norm_dx_wide(const NormArgs p) {
     const int64_t g = r / p.group;
     auto gain = [&](int c) {
       float a = 1.f;
-      if (p.a) load_params<1>(p.a, p.p_type, g * p.a_stride + c, false, &a);
+      if (p.a) a = load_param(p.a, p.p_type, g * p.a_stride + c);
       return p.one_plus ? a + 1.f : a;
     };
     float2 s = make_float2(0.f, 0.f);
@@ -785,7 +971,7 @@ __global__ void __launch_bounds__(1024) k_norm_dx_wide(const NormArgs p) {
       s.x += d;
       s.y = fmaf(d, (to_f(x[c]) - mu) * rs, s.y);
     }
-    s = team_sum2<1024>(s, red[flip]);
+    s = Wide::sum2(s, red[flip]);
     flip ^= 1;
     const float m1 = s.x * inv_n, m2 = s.y * inv_n;
     T* o = static_cast<T*>(p.out) + r * p.width;
@@ -803,15 +989,22 @@ __global__ void __launch_bounds__(256) k_norm_sums_wide(const NormArgs p) {
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (col >= p.width) return;
   for (int64_t item = blockIdx.y; item < p.items; item += gridDim.y) {
-    const Item it = item_rows(p, item);
+    const Item it = item_rows<1>(p, item, 0);
     float a = 0.f, b = 0.f;
-    for (int64_t r = it.r0; r < it.r1; ++r) {
+    for (int64_t r = it.first; r < it.end; r += it.step) {
       const float g = to_f(static_cast<const T*>(p.dy)[r * p.dy_stride + col]);
       const float z = (to_f(static_cast<const T*>(p.x)[r * p.x_stride + col]) - p.stats[r]) * p.stats[p.rows + r];
       a = fmaf(g, z, a);
       b += g;
     }
-    store_sums<1>(p, item, it.g, col, false, &a, &b);
+    if (p.split > 1) {
+      float* w = p.ws + item * 2 * p.width + col;
+      w[0] = a;
+      w[p.width] = b;
+    } else {
+      if (p.da) store_param(p.da, p.p_type, it.g * p.width + col, a);
+      if (p.db) store_param(p.db, p.p_type, it.g * p.width + col, b);
+    }
   }
 }
 
@@ -846,12 +1039,10 @@ void cut_items(NormArgs* p, int x_type, bool backward) {
     // A team's items where a group has too few rows to keep a block's teams busy and there
     // are groups enough to fill the GPU without splitting them.
     p->team_items = p->group < 2 * t.teams && groups >= 2 * kSms;
-    const int64_t want = (full_grid(t.tpr, backward) + groups - 1) / groups;
+    const int64_t want = full_grid(t.tpr, backward) / groups;  // one wave of blocks
     const int64_t most = (p->group + t.teams - 1) / t.teams;
     p->split = p->team_items ? 1 : (int)std::max<int64_t>(1, std::min(want, most));
   }
-  p->chunk = (p->group + p->split - 1) / p->split;
-  p->split = (int)((p->group + p->chunk - 1) / p->chunk);  // no empty item
   p->items = groups * p->split;
 }
 
@@ -885,51 +1076,50 @@ cudaError_t launch_ring(K kern, bool* raised, int64_t grid, int threads, int sme
   return launch_k(kern, dim3((unsigned)grid), dim3(threads), smem, st, p);
 }
 
-template <typename T, int E, int NV, int TPR>
+template <typename T, typename Tm>
 cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
-  using St = Stage<T, E, NV, TPR>;
   static bool raised[2][64];  // only ever set to true: calls from several threads may repeat the attribute
-  const int bytes = (backward ? 2 : 1) * St::BYTES;
-  p.stages = ring_stages(bytes, bound_blocks(TPR, backward));
-  const int64_t blocks = p.team_items ? (p.items + St::TEAMS - 1) / St::TEAMS : p.items;
-  const int64_t grid = std::min(blocks, full_grid(TPR, backward));
-  return backward ? launch_ring(k_norm_bwd<T, E, NV, TPR>, raised[1], grid, St::THREADS, bytes * p.stages, p, st)
-                  : launch_ring(k_norm_fwd<T, E, NV, TPR>, raised[0], grid, St::THREADS, bytes * p.stages, p, st);
+  const int bytes = (backward ? 2 : 1) * Stage<T, Tm>::BYTES;
+  p.stages = ring_stages(bytes, bound_blocks(Tm::TPR, backward));
+  const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
+  const int64_t grid = std::min(blocks, full_grid(Tm::TPR, backward));
+  return backward ? launch_ring(k_norm_bwd<T, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
+                  : launch_ring(k_norm_fwd<T, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
 }
 
 // group 1: the modulation in the ring, if two stages of it fit.
-template <typename T, typename P, int E, int NV, int TPR>
+template <typename T, typename P, typename Tm>
 cudaError_t launch_rowmod(NormArgs p, bool backward, cudaStream_t st) {
-  using St = Stage<T, E, NV, TPR>;
-  using Sp = Stage<P, E, NV, TPR>;
   static bool raised[2][64];
-  const int bytes = backward ? 2 * St::BYTES + Sp::BYTES : St::BYTES + 2 * Sp::BYTES;
-  p.stages = ring_stages(bytes, bound_blocks(TPR, false));
-  if (p.stages == 0) return launch_items<T, E, NV, TPR>(p, backward, st);
-  const int64_t grid = std::min((p.rows + St::TEAMS - 1) / St::TEAMS, full_grid(TPR, false));
-  return backward ? launch_ring(k_rowmod_bwd<T, P, E, NV, TPR>, raised[1], grid, St::THREADS, bytes * p.stages, p, st)
-                  : launch_ring(k_rowmod_fwd<T, P, E, NV, TPR>, raised[0], grid, St::THREADS, bytes * p.stages, p, st);
+  const int x_bytes = Stage<T, Tm>::BYTES, p_bytes = Stage<P, Tm>::BYTES;
+  const int bytes = backward ? 2 * x_bytes + p_bytes : x_bytes + 2 * p_bytes;
+  p.stages = ring_stages(bytes, bound_blocks(Tm::TPR, backward));
+  if (p.stages == 0) return launch_items<T, Tm>(p, backward, st);
+  const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, full_grid(Tm::TPR, backward));
+  return backward ? launch_ring(k_rowmod_bwd<T, P, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
+                  : launch_ring(k_rowmod_fwd<T, P, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
 }
 
 template <typename T, int E, int NV, int TPR>
 cudaError_t launch_tier(const NormArgs& p, bool backward, cudaStream_t st) {
-  if (p.group > 1 || !p.one_plus) return launch_items<T, E, NV, TPR>(p, backward, st);
-  if (p.p_type == LEWM_TYPE_F32) return launch_rowmod<T, float, E, NV, TPR>(p, backward, st);
+  using Tm = Team<E, NV, TPR>;
+  if (p.group > 1 || !p.one_plus) return launch_items<T, Tm>(p, backward, st);
+  if (p.p_type == LEWM_TYPE_F32) return launch_rowmod<T, float, Tm>(p, backward, st);
   constexpr bool any = std::is_same<T, float>::value;
   if constexpr (any || std::is_same<T, __nv_bfloat16>::value)
-    if (p.p_type == LEWM_TYPE_BF16) return launch_rowmod<T, __nv_bfloat16, E, NV, TPR>(p, backward, st);
+    if (p.p_type == LEWM_TYPE_BF16) return launch_rowmod<T, __nv_bfloat16, Tm>(p, backward, st);
   if constexpr (any || std::is_same<T, __half>::value)
-    if (p.p_type == LEWM_TYPE_F16) return launch_rowmod<T, __half, E, NV, TPR>(p, backward, st);
-  return launch_items<T, E, NV, TPR>(p, backward, st);  // bf16 beside fp16
+    if (p.p_type == LEWM_TYPE_F16) return launch_rowmod<T, __half, Tm>(p, backward, st);
+  return launch_items<T, Tm>(p, backward, st);  // bf16 beside fp16
 }
 
 template <typename T, int E>
 cudaError_t launch_width(const NormArgs& p, bool backward, cudaStream_t st) {
-  constexpr int E8 = E, V8 = 8 / E, V16 = 16 / E;
+  constexpr int V8 = 8 / E, V16 = 16 / E;
   switch (tier_of(p.width).tpr) {
-    case 8: return launch_tier<T, E8, V8, 8>(p, backward, st);
+    case 8: return launch_tier<T, E, V8, 8>(p, backward, st);
     case 32:
-      return p.width <= 256 ? launch_tier<T, E8, V8, 32>(p, backward, st) : launch_tier<T, E8, V16, 32>(p, backward, st);
+      return p.width <= 256 ? launch_tier<T, E, V8, 32>(p, backward, st) : launch_tier<T, E, V16, 32>(p, backward, st);
     case 64: return launch_tier<T, E, V16, 64>(p, backward, st);
     case 128: return launch_tier<T, E, V16, 128>(p, backward, st);
     case 256: return launch_tier<T, E, V16, 256>(p, backward, st);
@@ -977,8 +1167,9 @@ cudaError_t launch_norm(NormArgs p, int x_type, bool backward, cudaStream_t st) 
                                              : launch_type<__half>(p, wide, backward, vec, st);
   if (e != cudaSuccess || !backward || p.split == 1 || (!p.da && !p.db)) return e;
   const int64_t groups = p.items / p.split;
-  const dim3 grid((unsigned)((p.width + 31) / 32), (unsigned)std::min<int64_t>(groups, 65535), 2);
-  return launch_k(k_norm_reduce, grid, dim3(32, 32), 0, st, p);
+  const unsigned gy = (unsigned)std::min<int64_t>(groups, 65535);
+  if (p.split <= 16) return launch_k(k_norm_reduce<1>, dim3((p.width + 255) / 256, gy, 2), dim3(256), 0, st, p);
+  return launch_k(k_norm_reduce<32>, dim3((p.width + 31) / 32, gy, 2), dim3(1024), 0, st, p);
 }
 
 lewm_status norm_fail(lewm_status s, const char* fmt, ...) {
