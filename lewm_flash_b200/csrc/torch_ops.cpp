@@ -9,6 +9,7 @@
 // its checks, 677 and 102 us.
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -279,13 +280,27 @@ float check_max_norm(double max_norm) {
   return static_cast<float>(max_norm);
 }
 
-void check_list(const char* name, const std::vector<Tensor>& ts) {
+// The tensors of a Python list, borrowed from it: converting a list through the binding's casters
+// took longer than all the checks.
+using Refs = std::vector<const Tensor*>;
+Refs refs(const char* name, const py::list& list) {
+  Refs out;
+  out.reserve(list.size());
+  for (py::handle h : list) {
+    TORCH_CHECK_TYPE(THPVariable_Check(h.ptr()), name, "[", out.size(), "] must be a tensor, got ",
+                     Py_TYPE(h.ptr())->tp_name);
+    out.push_back(&THPVariable_Unpack(h.ptr()));
+  }
+  return out;
+}
+
+void check_list(const char* name, const Refs& ts) {
   for (size_t i = 0; i < ts.size(); ++i) {
-    const Tensor& t = ts[i];
+    const Tensor& t = *ts[i];
     if (type_code(t) < 0 || t.layout() != at::kStrided)
       check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
-    TORCH_CHECK_VALUE(t.device() == ts[0].device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
-                      ts[0].device(), ": one device per call");
+    TORCH_CHECK_VALUE(t.device() == ts[0]->device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
+                      ts[0]->device(), ": one device per call");
   }
 }
 
@@ -312,18 +327,17 @@ bool overlap(const std::vector<int64_t>& src, const std::vector<int64_t>& dst, c
 }
 
 // The kernels' call: norm of dense `src`, and with `dst` their scaled copies.
-Tensor clip(const std::vector<Tensor>& src, const std::vector<Tensor>* dst, float max_norm, int kind,
-            const Tensor& norm_in) {
+Tensor clip(const Refs& src, const Refs* dst, float max_norm, int kind, const Tensor& norm_in) {
   const size_t n = src.size();
   std::vector<const void*> sp(n);
   std::vector<void*> dp(dst ? n : 0);
   std::vector<int64_t> count(n);
   std::vector<int32_t> type(n);
   for (size_t i = 0; i < n; ++i) {
-    count[i] = src[i].numel();
-    type[i] = type_code(src[i]);
-    sp[i] = src[i].const_data_ptr();
-    if (dst) dp[i] = (*dst)[i].mutable_data_ptr();
+    count[i] = src[i]->numel();
+    type[i] = type_code(*src[i]);
+    sp[i] = src[i]->const_data_ptr();
+    if (dst) dp[i] = (*dst)[i]->mutable_data_ptr();
   }
   if (dst) {
     std::vector<int64_t> s(n), d(n), size(n);
@@ -335,11 +349,11 @@ Tensor clip(const std::vector<Tensor>& src, const std::vector<Tensor>* dst, floa
     TORCH_CHECK_VALUE(!overlap(s, d, size),
                       "gradients overlap in memory (the same one listed twice?), or an output overlaps one");
   }
-  need_cuda(src[0]);
-  const auto opt = src[0].options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+  need_cuda(*src[0]);
+  const auto opt = src[0]->options().requires_grad(false).dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
   Tensor norm = at::empty({}, opt), ws = at::empty({LEWM_GRAD_WORKSPACE}, opt.dtype(at::kByte));
-  const int device = src[0].get_device();
-  void* stream = stream_of(src[0]);
+  const int device = src[0]->get_device();
+  void* stream = stream_of(*src[0]);
   float* out = static_cast<float*>(norm.mutable_data_ptr());
   const int32_t m = static_cast<int32_t>(std::min<size_t>(n, std::numeric_limits<int32_t>::max()));
   if (!dst) check_status(lewm_grad_norm(sp.data(), count.data(), type.data(), m, kind, mut(ws), out, device, stream));
@@ -349,10 +363,15 @@ Tensor clip(const std::vector<Tensor>& src, const std::vector<Tensor>* dst, floa
   return norm;
 }
 
-std::vector<Tensor> dense(const std::vector<Tensor>& ts) {
-  std::vector<Tensor> out;
-  out.reserve(ts.size());
-  for (const Tensor& t : ts) out.push_back(t.contiguous());  // the tensor itself where it is contiguous
+// `ts` with contiguous copies, held in `copies`, in the place of those that are not.
+Refs dense(const Refs& ts, std::vector<Tensor>* copies) {
+  Refs out = ts;
+  copies->reserve(ts.size());  // the addresses of its elements stay
+  for (size_t i = 0; i < ts.size(); ++i) {
+    if (ts[i]->is_contiguous()) continue;
+    copies->push_back(ts[i]->contiguous());
+    out[i] = &copies->back();
+  }
   return out;
 }
 
@@ -361,64 +380,67 @@ void bump(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-Tensor grad_norm(const std::vector<Tensor>& grads, double norm_type) {
+Tensor grad_norm(const py::list& list, double norm_type) {
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
+  const Refs grads = refs("grads", list);
   if (grads.empty()) return at::zeros({}, at::kFloat);
   check_list("grads", grads);
-  return clip(dense(grads), nullptr, 0.f, kind, Tensor());
+  std::vector<Tensor> copies;
+  return clip(dense(grads, &copies), nullptr, 0.f, kind, Tensor());
 }
 
-std::pair<std::vector<Tensor>, Tensor> clip_grads(const std::vector<Tensor>& grads, double max_norm, double norm_type,
-                                                  const std::optional<std::vector<Tensor>>& out_given) {
+std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, double norm_type,
+                                       const std::optional<py::list>& out_given) {
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   const float limit = check_max_norm(max_norm);
-  std::vector<Tensor> out;
-  if (out_given) {
-    out = *out_given;
-    TORCH_CHECK_VALUE(out.size() == grads.size(), "out has ", out.size(), " tensors, grads ", grads.size());
-  }
-  if (grads.empty()) return {out, at::zeros({}, at::kFloat)};
+  const Refs grads = refs("grads", list);
+  py::list out_list = out_given ? *out_given : py::list();
+  if (out_given)
+    TORCH_CHECK_VALUE(out_list.size() == grads.size(), "out has ", out_list.size(), " tensors, grads ", grads.size());
+  if (grads.empty()) return {out_list, at::zeros({}, at::kFloat)};
   check_list("grads", grads);
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const Tensor& g = grads[i];
-    if (!out_given) {
-      out.push_back(at::empty(g.sizes(), g.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)));
-      continue;
-    }
-    const Tensor& o = out[i];
+  if (!out_given)
+    for (const Tensor* g : grads)
+      out_list.append(
+          at::empty(g->sizes(), g->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)));
+  const Refs out = refs("out", out_list);
+  for (size_t i = 0; out_given && i < grads.size(); ++i) {
+    const Tensor &g = *grads[i], &o = *out[i];
     TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
                           o.device() == g.device(),
                       "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
     TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");
   }
-  Tensor norm = clip(dense(grads), &out, limit, kind, Tensor());
+  std::vector<Tensor> copies;
+  Tensor norm = clip(dense(grads, &copies), &out, limit, kind, Tensor());
   if (out_given)
-    for (const Tensor& o : out) bump(o);
-  return {std::move(out), std::move(norm)};
+    for (const Tensor* o : out) bump(*o);
+  return {std::move(out_list), std::move(norm)};
 }
 
-Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double norm_type, bool error_if_nonfinite) {
+Tensor clip_in_place(const py::list& list, double max_norm, double norm_type, bool error_if_nonfinite) {
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   const float limit = check_max_norm(max_norm);
+  const Refs grads = refs("grad", list);
   if (grads.empty()) return at::zeros({}, at::kFloat);
-  check_list("grads", grads);
-  std::vector<size_t> strided;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const Tensor& g = grads[i];
-    if (g.is_contiguous()) continue;
-    for (int64_t d = 0; d < g.dim(); ++d)
-      TORCH_CHECK_VALUE(g.stride(d) != 0 || g.size(d) <= 1, "a gradient of shape ", g.sizes(),
+  check_list("grad", grads);
+  Refs strided;
+  for (const Tensor* g : grads) {
+    if (g->is_contiguous()) continue;
+    for (int64_t d = 0; d < g->dim(); ++d)
+      TORCH_CHECK_VALUE(g->stride(d) != 0 || g->size(d) <= 1, "a gradient of shape ", g->sizes(),
                         " shares memory between its own elements");
-    for (size_t j : strided)
-      TORCH_CHECK_VALUE(!(grads[j].const_data_ptr() == g.const_data_ptr() && grads[j].sizes() == g.sizes() &&
-                          grads[j].strides() == g.strides()),
+    for (const Tensor* o : strided)
+      TORCH_CHECK_VALUE(!(o->const_data_ptr() == g->const_data_ptr() && o->sizes() == g->sizes() &&
+                          o->strides() == g->strides()),
                         "gradients overlap in memory (the same one listed twice?)");
-    strided.push_back(i);
+    strided.push_back(g);
   }
-  const std::vector<Tensor> ts = dense(grads);
+  std::vector<Tensor> copies;
+  const Refs ts = dense(grads, &copies);
   Tensor norm_in;
   if (error_if_nonfinite) {
     norm_in = clip(ts, nullptr, 0.f, kind, Tensor());
@@ -426,9 +448,9 @@ Tensor clip_in_place(const std::vector<Tensor>& grads, double max_norm, double n
                 " for gradients is non-finite, so it cannot be clipped");
   }
   Tensor norm = clip(ts, &ts, limit, kind, norm_in);
-  for (size_t i : strided) grads[i].copy_(ts[i]);  // counts as a change by itself
-  for (const Tensor& g : grads)
-    if (g.is_contiguous()) bump(g);
+  for (size_t i = 0; i < strided.size(); ++i) strided[i]->copy_(copies[i]);  // counts as a change by itself
+  for (const Tensor* g : grads)
+    if (g->is_contiguous()) bump(*g);
   return norm;
 }
 

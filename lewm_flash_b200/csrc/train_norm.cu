@@ -69,6 +69,7 @@ struct NormArgs {
   int64_t group;       // rows per (a, b)
   int64_t items;       // groups * split
   int split;           // items per group
+  int loop_min, loop_rem;  // a loop that starts `o` rows into its rows has loop_min + (o < loop_rem) rounds
   int width;
   int p_type;
   int one_plus;        // a = 1 + a[]
@@ -443,24 +444,33 @@ struct Stage {
 // front: with a contiguous run of rows for each block DRAM gave less (73881 x 1536 float32
 // backward: 4.3 against 6.4 TB/s).
 struct Item {
-  int64_t g, first, end, step;
-  int64_t iters;  // of the whole block's loop
+  int64_t g, first, step;
+  int rows, iters;  // of this team; of the whole block's loop
 };
 template <int TEAMS>
 __device__ __forceinline__ Item item_rows(const NormArgs& p, int64_t base, int team) {
-  Item it{0, 0, 0, 1, p.group};
+  Item it{0, 0, 1, 0, p.loop_min};
   if (p.team_items) {
     it.g = base + team;
-    if (it.g >= p.items) return Item{0, 0, 0, 1, p.group};  // no rows
+    it.rows = it.g < p.items ? p.loop_min : 0;
     it.first = it.g * p.group;
   } else {
-    it.g = p.split == 1 ? base : base / p.split;
-    const int64_t s = base - it.g * p.split;
+    int s = 0;
+    if (p.split == p.items) s = (int)base;  // one group
+    else if (p.split == 1) it.g = base;
+    else if (p.items <= UINT_MAX) {
+      it.g = (uint32_t)base / (uint32_t)p.split;
+      s = (int)((uint32_t)base - (uint32_t)it.g * (uint32_t)p.split);
+    } else {
+      it.g = base / p.split;
+      s = (int)(base - it.g * p.split);
+    }
+    const int64_t o = (int64_t)s * TEAMS;
     it.step = (int64_t)p.split * TEAMS;
-    it.first = it.g * p.group + s * TEAMS + team;
-    it.iters = (p.group - s * TEAMS + it.step - 1) / it.step;
+    it.first = it.g * p.group + o + team;
+    it.iters = p.loop_min + (o < p.loop_rem);
+    it.rows = p.loop_min + (o + team < p.loop_rem);
   }
-  it.end = (it.g + 1) * p.group;
   return it;
 }
 
@@ -477,9 +487,15 @@ struct Walk {
         step(step_rows * stride) {}
 };
 
-// Blocks per SM that the registers are limited for: 80 a thread forward, 128 backward.
-constexpr int bound_blocks(int tpr, bool backward) {
-  const int n = (backward ? 512 : 768) / block_threads(tpr);
+// Blocks per SM that the registers are limited for: 80 a thread forward, 128 in the backward that
+// keeps sums. More, smaller blocks were slower on short rows (16448 x 192 bf16 forward, 3, 4 and 5
+// blocks: 6.8, 6.9, 7.2 us): every block loads the parameters anew. The backward of a modulation
+// row per row has neither and takes 4 there (57600 x 192 bf16, 2, 3 and 4 blocks: 26.2, 22.9,
+// 21.6 us).
+template <typename Tm>
+constexpr int bound_blocks(bool backward, bool rowmod = false) {
+  if (rowmod && backward && Tm::N == 8) return 4;
+  const int n = (backward ? 512 : 768) / Tm::THREADS;
   return n > 0 ? n : 1;
 }
 
@@ -515,7 +531,7 @@ __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float
 }
 
 template <typename T, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_norm_fwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_norm_fwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
   using St = Stage<T, Tm>;
   constexpr int H = Tm::H;
@@ -528,7 +544,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_n
     const Item it = item_rows<Tm::TEAMS>(p, base, Tm::team());
     Walk<T> x(p.x, p.rows, p.x_stride, p.width, it.first, it.step);
     const T* x_now = x.at;  // the row being computed; x.at is the one being fetched
-    int64_t left = it.first < it.end ? (it.end - it.first + it.step - 1) / it.step : 0, ahead = left;
+    int left = it.rows, ahead = left;
     uint32_t in = ring0, out = ring0;
     auto fetch = [&]() {
       if (ahead > 0) St::fetch(in, x.at, p.width, x.lo, x.hi);
@@ -551,7 +567,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_n
     }
     int64_t r = it.first;
     T* y = static_cast<T*>(p.out) + r * p.width;
-    for (int64_t k = 0; k < it.iters; ++k) {
+    for (int k = 0; k < it.iters; ++k) {
       cp_wait(p.stages);
       if constexpr (Tm::E == 1) Tm::barrier();
       fetch();
@@ -585,7 +601,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_n
 
 // A modulation row per row of x: rows in a grid stride, scale and shift in the ring beside x.
 template <typename T, typename P, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_rowmod_fwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_rowmod_fwd(const NormArgs p) {
   griddep_wait();
   using St = Stage<T, Tm>;
   using Sp = Stage<P, Tm>;
@@ -595,12 +611,12 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_r
   const float inv_n = 1.0f / p.width;
   const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
   const int64_t first = (int64_t)blockIdx.x * Tm::TEAMS + Tm::team(), step = (int64_t)gridDim.x * Tm::TEAMS;
-  const int64_t iters = (p.rows - (int64_t)blockIdx.x * Tm::TEAMS + step - 1) / step;
+  const int iters = p.loop_min + ((int64_t)blockIdx.x * Tm::TEAMS < p.loop_rem);
   Walk<T> x(p.x, p.rows, p.x_stride, p.width, first, step);
   Walk<P> a(p.a, p.rows, p.a_stride, p.width, first, step), b(p.b, p.rows, p.b_stride, p.width, first, step);
   const T* x_now = x.at;
   const P *a_now = a.at, *b_now = b.at;
-  int64_t left = first < p.rows ? (p.rows - first + step - 1) / step : 0, ahead = left;
+  int left = p.loop_min + (first < p.loop_rem), ahead = left;
   uint32_t in = ring0, out = ring0;
   auto fetch = [&]() {
     if (ahead > 0) {
@@ -616,7 +632,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, false)) k_r
   for (int k = 0; k < p.stages - 1; ++k) fetch();
   int64_t r = first;
   T* y = static_cast<T*>(p.out) + r * p.width;
-  for (int64_t k = 0; k < iters; ++k) {
+  for (int k = 0; k < iters; ++k) {
     cp_wait(p.stages);
     if constexpr (Tm::E == 1) Tm::barrier();
     fetch();
@@ -661,7 +677,7 @@ __device__ __forceinline__ void store_dx(T* dx, int width, const F2* z, F2* d, f
 }
 
 template <typename T, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_norm_bwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true)) k_norm_bwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
   // The whole grid is resident by now, so the reduction's blocks take no slot from it; they
   // wait for its end with their launch behind them.
@@ -683,7 +699,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_no
     Walk<T> x(p.x, p.rows, p.x_stride, p.width, it.first, it.step);
     Walk<T> dy(p.dy, p.rows, p.dy_stride, p.width, it.first, it.step);
     const T *x_now = x.at, *dy_now = dy.at;
-    int64_t left = it.first < it.end ? (it.end - it.first + it.step - 1) / it.step : 0, ahead = left;
+    int left = it.rows, ahead = left;
     const bool any = left > 0;
     uint32_t in = ring0, out = ring0;
     auto fetch = [&]() {
@@ -710,7 +726,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_no
     float mu = 0.f, rs = 0.f;
     if (any) mu = stat[0], rs = stat[p.rows];
     T* dx = static_cast<T*>(p.out) + it.first * p.width;
-    for (int64_t k = 0; k < it.iters; ++k) {
+    for (int k = 0; k < it.iters; ++k) {
       cp_wait(p.stages);
       if constexpr (E == 1) Tm::barrier();
       fetch();
@@ -799,7 +815,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_no
 
 // A modulation row per row of x: d scale = dy z and d shift = dy row by row, nothing to sum up.
 template <typename T, typename P, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_rowmod_bwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true, true)) k_rowmod_bwd(const NormArgs p) {
   griddep_wait();
   using St = Stage<T, Tm>;
   using Sp = Stage<P, Tm>;
@@ -809,12 +825,12 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_ro
   const float inv_n = 1.0f / p.width;
   const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
   const int64_t first = (int64_t)blockIdx.x * Tm::TEAMS + Tm::team(), step = (int64_t)gridDim.x * Tm::TEAMS;
-  const int64_t iters = (p.rows - (int64_t)blockIdx.x * Tm::TEAMS + step - 1) / step;
+  const int iters = p.loop_min + ((int64_t)blockIdx.x * Tm::TEAMS < p.loop_rem);
   Walk<T> x(p.x, p.rows, p.x_stride, p.width, first, step), dy(p.dy, p.rows, p.dy_stride, p.width, first, step);
   Walk<P> a(p.a, p.rows, p.a_stride, p.width, first, step);
   const T *x_now = x.at, *dy_now = dy.at;
   const P* a_now = a.at;
-  int64_t left = first < p.rows ? (p.rows - first + step - 1) / step : 0, ahead = left;
+  int left = p.loop_min + (first < p.loop_rem), ahead = left;
   uint32_t in = ring0, out = ring0;
   auto fetch = [&]() {
     if (ahead > 0) {
@@ -833,7 +849,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_ro
   if (left > 0) mu = stat[0], rs = stat[p.rows];
   int64_t at = first * p.width;
   int flip = 0;
-  for (int64_t k = 0; k < iters; ++k) {
+  for (int k = 0; k < iters; ++k) {
     cp_wait(p.stages);
     if constexpr (Tm::E == 1) Tm::barrier();
     fetch();
@@ -879,39 +895,59 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks(Tm::TPR, true)) k_ro
   }
 }
 
-// Sum of the `split` partial sums of each group in a fixed order: R interleaved runs of items, then
-// the runs. 32 columns x R runs per block, grid (column tiles, groups, a or b); with R = 1 a
-// thread adds a column's few partials by itself and 8 column tiles share a block.
-template <int R>
-__global__ void __launch_bounds__(R > 1 ? 32 * R : 256) k_norm_reduce(const NormArgs p) {
+// Sum of the `split` partial sums of each group in a fixed order. R = 32: 32 interleaved runs of
+// items by 8 vectors of VW columns in a block, all of a run's loads started together, then the
+// runs through shared memory. R = 1, for few items: a thread adds a vector's partials by itself.
+// Grid (column tiles, groups, a or b).
+template <int R, int VW>
+__global__ void __launch_bounds__(256) k_norm_reduce(const NormArgs p) {
   griddep_wait();
-  __shared__ float part[R][33];
-  constexpr int COLS = R > 1 ? 32 : 256;
-  const int cx = R > 1 ? threadIdx.x % 32 : threadIdx.x, run = R > 1 ? threadIdx.x / 32 : 0;
-  const int64_t col = (int64_t)blockIdx.x * COLS + cx;
+  constexpr int LANES = 256 / R, COLS = LANES * VW;
+  using V = Vec<float, VW>;
+  __shared__ V part[R][LANES];
+  const int cx = threadIdx.x % LANES, run = threadIdx.x / LANES;
+  const int64_t col = (int64_t)blockIdx.x * COLS + cx * VW;
   void* out = blockIdx.z ? p.db : p.da;
   if (!out) return;
-  const int64_t groups = p.items / p.split;
+  const int64_t groups = p.items / p.split, stride = 2 * (int64_t)p.width;
   for (int64_t g = blockIdx.y; g < groups; g += gridDim.y) {
-    float s = 0.f;
+    V s;
+#pragma unroll
+    for (int e = 0; e < VW; ++e) s.v[e] = 0.f;
     if (col < p.width) {
       const float* w = p.ws + (g * p.split * 2 + blockIdx.z) * p.width + col;
-#pragma unroll 8
-      for (int i = run; i < p.split; i += R) s += w[(int64_t)i * 2 * p.width];
+      for (int i = run; i < p.split; i += 8 * R) {
+        V v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i + k * R < p.split) v[k] = *reinterpret_cast<const V*>(w + (i + k * R) * stride);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i + k * R < p.split) {
+#pragma unroll
+            for (int e = 0; e < VW; ++e) s.v[e] += v[k].v[e];
+          }
+      }
     }
-    if constexpr (R == 1) {
-      if (col < p.width) store_param(out, p.p_type, g * p.width + col, s);
-    } else {
+    if constexpr (R > 1) {
       part[run][cx] = s;
       __syncthreads();
-      if (run == 0 && col < p.width) {
-        float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < R; ++i) t += part[i][cx];
-        store_param(out, p.p_type, g * p.width + col, t);
+      for (int half = R / 2; half > 0; half >>= 1) {
+        if (run < half) {
+#pragma unroll
+          for (int e = 0; e < VW; ++e) part[run][cx].v[e] += part[run + half][cx].v[e];
+        }
+        if (half * LANES > 32) __syncthreads();
+        else __syncwarp();
       }
-      __syncthreads();
+      s = part[0][cx];
     }
+    if (run == 0 && col < p.width) {
+#pragma unroll
+      for (int e = 0; e < VW; ++e) store_param(out, p.p_type, g * p.width + col + e, s.v[e]);
+    }
+    if (R > 1) __syncthreads();
   }
 }
 
@@ -991,7 +1027,8 @@ __global__ void __launch_bounds__(256) k_norm_sums_wide(const NormArgs p) {
   for (int64_t item = blockIdx.y; item < p.items; item += gridDim.y) {
     const Item it = item_rows<1>(p, item, 0);
     float a = 0.f, b = 0.f;
-    for (int64_t r = it.first; r < it.end; r += it.step) {
+    int64_t r = it.first;
+    for (int k = 0; k < it.rows; ++k, r += it.step) {
       const float g = to_f(static_cast<const T*>(p.dy)[r * p.dy_stride + col]);
       const float z = (to_f(static_cast<const T*>(p.x)[r * p.x_stride + col]) - p.stats[r]) * p.stats[p.rows + r];
       a = fmaf(g, z, a);
@@ -1023,7 +1060,19 @@ Tier tier_of(int64_t width) {
 int64_t type_size(int type) { return type == LEWM_TYPE_F32 ? 4 : 2; }
 bool is_wide(const NormArgs& p, int x_type) { return p.width * type_size(x_type) > kMaxRowBytes; }
 
-int64_t full_grid(int tpr, bool backward) { return (int64_t)kSms * bound_blocks(tpr, backward); }
+// Blocks that fill the GPU once.
+int64_t full_grid(const Tier& t, bool backward) {
+  return (int64_t)kSms * (t.tpr <= 256   ? bound_blocks<Team<1, 16, 32>>(backward)
+                          : t.tpr == 512 ? bound_blocks<Team<1, 16, 512>>(backward)
+                                         : bound_blocks<Team<1, 16, 1024>>(backward));
+}
+
+// Rounds of loops over `rows` rows in steps of `step`. (No tensor that fits a GPU makes 2^31 rounds: a
+// step is a row for groups of a few, else a block's teams times the blocks that share the rows.)
+void set_loop(NormArgs* p, int64_t rows, int64_t step) {
+  p->loop_min = (int)std::min<int64_t>(rows / step, INT_MAX - 1);
+  p->loop_rem = (int)(rows % step);
+}
 
 // How rows are cut into items; the same function sizes the workspace.
 void cut_items(NormArgs* p, int x_type, bool backward) {
@@ -1039,11 +1088,12 @@ void cut_items(NormArgs* p, int x_type, bool backward) {
     // A team's items where a group has too few rows to keep a block's teams busy and there
     // are groups enough to fill the GPU without splitting them.
     p->team_items = p->group < 2 * t.teams && groups >= 2 * kSms;
-    const int64_t want = full_grid(t.tpr, backward) / groups;  // one wave of blocks
+    const int64_t want = full_grid(t, backward) / groups;  // one wave of blocks
     const int64_t most = (p->group + t.teams - 1) / t.teams;
     p->split = p->team_items ? 1 : (int)std::max<int64_t>(1, std::min(want, most));
   }
   p->items = groups * p->split;
+  set_loop(p, p->group, p->team_items ? 1 : (int64_t)p->split * (is_wide(*p, x_type) ? 1 : tier_of(p->width).teams));
 }
 
 size_t workspace_bytes(const NormArgs& p) {
@@ -1080,9 +1130,9 @@ template <typename T, typename Tm>
 cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
   static bool raised[2][64];  // only ever set to true: calls from several threads may repeat the attribute
   const int bytes = (backward ? 2 : 1) * Stage<T, Tm>::BYTES;
-  p.stages = ring_stages(bytes, bound_blocks(Tm::TPR, backward));
+  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward));
   const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
-  const int64_t grid = std::min(blocks, full_grid(Tm::TPR, backward));
+  const int64_t grid = std::min(blocks, (int64_t)kSms * bound_blocks<Tm>(backward));
   return backward ? launch_ring(k_norm_bwd<T, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
                   : launch_ring(k_norm_fwd<T, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
 }
@@ -1093,9 +1143,10 @@ cudaError_t launch_rowmod(NormArgs p, bool backward, cudaStream_t st) {
   static bool raised[2][64];
   const int x_bytes = Stage<T, Tm>::BYTES, p_bytes = Stage<P, Tm>::BYTES;
   const int bytes = backward ? 2 * x_bytes + p_bytes : x_bytes + 2 * p_bytes;
-  p.stages = ring_stages(bytes, bound_blocks(Tm::TPR, backward));
+  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward, true));
   if (p.stages == 0) return launch_items<T, Tm>(p, backward, st);
-  const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, full_grid(Tm::TPR, backward));
+  const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, (int64_t)kSms * bound_blocks<Tm>(backward, true));
+  set_loop(&p, p.rows, grid * Tm::TEAMS);
   return backward ? launch_ring(k_rowmod_bwd<T, P, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
                   : launch_ring(k_rowmod_fwd<T, P, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
 }
@@ -1168,8 +1219,13 @@ cudaError_t launch_norm(NormArgs p, int x_type, bool backward, cudaStream_t st) 
   if (e != cudaSuccess || !backward || p.split == 1 || (!p.da && !p.db)) return e;
   const int64_t groups = p.items / p.split;
   const unsigned gy = (unsigned)std::min<int64_t>(groups, 65535);
-  if (p.split <= 16) return launch_k(k_norm_reduce<1>, dim3((p.width + 255) / 256, gy, 2), dim3(256), 0, st, p);
-  return launch_k(k_norm_reduce<32>, dim3((p.width + 31) / 32, gy, 2), dim3(1024), 0, st, p);
+  const int vw = p.width % 4 == 0 ? 4 : 1, cols = (p.split <= 16 ? 256 : 8) * vw;
+  const dim3 grid((p.width + cols - 1) / cols, gy, 2);
+  if (p.split <= 16)
+    return vw == 4 ? launch_k(k_norm_reduce<1, 4>, grid, dim3(256), 0, st, p)
+                   : launch_k(k_norm_reduce<1, 1>, grid, dim3(256), 0, st, p);
+  return vw == 4 ? launch_k(k_norm_reduce<32, 4>, grid, dim3(256), 0, st, p)
+                 : launch_k(k_norm_reduce<32, 1>, grid, dim3(256), 0, st, p);
 }
 
 lewm_status norm_fail(lewm_status s, const char* fmt, ...) {
