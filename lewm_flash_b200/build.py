@@ -18,7 +18,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "liblewm_b200.so"
 SOURCES = ["api.cu", "rollout_kernels.cu", "tile_call.cu", "fp32_path.cu", "icem_kernels.cu", "noalloc.cu", "encoder.cu",
            "train_norm.cu", "grad_clip.cu"]
-HEADERS = ["lewm_common.cuh", "lewm_internal.h"]
+HEADERS = ["lewm_common.cuh", "lewm_internal.h", "train_elem.cuh"]
 EXT = PKG / "_torch_ops.so"
 EXT_SOURCES = ["torch_ops.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -6,18 +6,16 @@
 // Bound: bytes. The norm reads every gradient once; the scaling cannot start before the norm
 // is known, so it reads them again (from L2 while they fit its 126 MB) and writes once.
 //
-// Layout: the tensors travel in the kernel's parameters (pointer, count, type and first chunk
-// of each: up to 32 KB, so no copy to the device and nothing a captured graph could find
-// changed). They are cut into chunks of 16 KB, four 16-byte loads for each of a block's 256
-// threads; persistent blocks take chunks in a fixed stride and look up a chunk's tensor by
-// bisection. Lists longer than a table take several launches that share the partial sums.
+// Layout: the tensors travel in the kernel's parameters (pointers, count, type and first chunk of
+// each: up to 32 KB, so no copy to the device and nothing a captured graph could find changed).
+// They are cut into chunks of a few 16-byte loads for each of a block's 256 threads; persistent
+// blocks take chunks in a fixed stride and look up a chunk's tensor by bisection. Lists longer
+// than a table take several launches that share the partial sums.
 //
-// The sum of squares of a 16-byte vector is float32 (at most 8 products of like sign) and joins
-// a float64 sum per thread; where that float32 sum is too small or too large for its squares
-// to be normal numbers the vector is summed again in float64. Each block
-// leaves one partial; the scaling blocks each add all partials in the same fixed order, which
-// saves a launch and needs no atomics: the same bits on every run.
-#include <cuda_fp16.h>
+// Squares are summed in float32 within a 16-byte vector (at most 8 terms of one sign) and in
+// float64 beyond; a chunk with squares outside the normal range of float32 is read again and
+// summed in float64. Each block leaves one partial; the scaling blocks each add all partials in
+// the same fixed order, which saves a launch and needs no atomics: the same bits on every run.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -25,19 +23,25 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "lewm_b200.h"
 #include "lewm_common.cuh"
 #include "lewm_internal.h"
+#include "train_elem.cuh"
 
 namespace lewm {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunkBytes = 16384;  // 4 vectors of 16 bytes per thread
-constexpr int kSlots = 2048;        // partial sums of all launches of a call
-constexpr int kBlocks = 148 * 8;    // 148 SMs x 8 blocks of 256 threads
-static_assert(kBlocks <= kSlots && kSlots * sizeof(double) + 16 <= LEWM_GRAD_WORKSPACE, "workspace");
+constexpr int kSms = 148;      // B200
+constexpr int kSlots = 2048;   // partial sums of all launches of a call
+// 16-byte vectors of a chunk per thread, all in flight at once, and blocks per SM. Norm of 2^28 bf16
+// elements with 8 x 4: 82 us (6.5 TB/s), 4 x 8: 101, 4 x 6: 94; norm and scaling with 4 x 4 for the
+// scaling: 275 us, 2 x 8: 290, 4 x 6: 297.
+constexpr int kNormVecs = 8, kNormBlocks = 4;
+constexpr int kScaleVecs = 4, kScaleBlocks = 4;
+static_assert(kSms * kNormBlocks <= kSlots && kSlots * sizeof(double) <= LEWM_GRAD_WORKSPACE, "workspace");
 
 // A launch's tensors. Element types and whether a tensor's vectors can be 16 bytes (src and
 // dst at the same offset from a 16-byte boundary) share a byte.
@@ -50,37 +54,32 @@ struct Table {
   uint8_t kind[N];        // LEWM_TYPE_* | 4 if only single elements can be moved
   int n;
 };
-constexpr int kSmall = 64, kLarge = 1024;
+constexpr int kSmall = 64, kMiddle = 256, kLarge = 1024;
 constexpr int kMaxTensors = 1 << 20;  // 1024 launches of the norm, each with a partial sum at least
 static_assert(sizeof(Table<kLarge>) + 64 <= 32764, "kernel parameters");
 
 // ------------------------------------------------------------------ a chunk of a tensor
-__device__ __forceinline__ float elem(float v) { return v; }
-__device__ __forceinline__ float elem(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float elem(__half v) { return __half2float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-
-// Elements of a chunk: a vector body [v0, v1) of 16-byte vectors counted from the tensor's
-// first 16-byte boundary (element `head`), and single elements [0, head) and [tail, count),
+// Elements of a chunk of VECS vectors per thread: 16-byte vectors [v0, v0 + vecs) counted from the
+// tensor's first 16-byte boundary (element `head`), and single elements [0, head) and [tail, count),
 // which belong to the first and the last chunk.
-template <typename T>
+template <typename T, int VECS>
 struct Span {
   static constexpr int E = 16 / sizeof(T);
-  int64_t head, body, v0, v1;  // body: vectors of the whole tensor
+  int64_t v0, tail;
+  int head, vecs;
   __device__ __forceinline__ Span(const T* p, int64_t count, uint32_t chunk) {
-    const int64_t off = (reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T);
-    head = min((E - off) % E, count);
-    body = (count - head) / E;
-    v0 = min((int64_t)chunk * (kChunkBytes / 16), body);
-    v1 = min(v0 + kChunkBytes / 16, body);
+    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15) / (int)sizeof(T);
+    head = (int)min((int64_t)((E - off) % E), count);
+    const int64_t body = (count - head) / E;
+    v0 = (int64_t)chunk * (kThreads * VECS);
+    vecs = (int)max((int64_t)0, min(body - v0, (int64_t)(kThreads * VECS)));
+    tail = head + body * E;
   }
 };
 
+// The tensor of a chunk, known to be one of [lo, hi).
 template <int N>
-__device__ __forceinline__ int find_tensor(const Table<N>& t, uint32_t chunk) {
-  int lo = 0, hi = t.n;  // first[lo] <= chunk < first[hi]
+__device__ __forceinline__ int find_tensor(const Table<N>& t, uint32_t chunk, int lo, int hi) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (t.first[mid] <= chunk) lo = mid;
@@ -96,57 +95,74 @@ template <bool MAX>
 struct Acc {
   double sum = 0.0;
   uint32_t bits = 0;
-  // K values; squares between 2^-100 and 2^126 summed in float32, others in float64.
-  template <int K>
-  __device__ __forceinline__ void add(const float* f) {
-    if constexpr (MAX) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) bits = max(bits, __float_as_uint(f[k]) & 0x7fffffffu);
-    } else {
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) s = fmaf(f[k], f[k], s);
-      if (s >= 0x1p-100f && s <= 0x1p126f) {
-        sum += (double)s;
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < K; ++k) sum = fma((double)f[k], (double)f[k], sum);
-      }
-    }
+  __device__ __forceinline__ void add(float f) {
+    if constexpr (MAX) bits = max(bits, __float_as_uint(f) & 0x7fffffffu);
+    else sum = fma((double)f, (double)f, sum);
   }
 };
 
+// This thread's vectors of a chunk added up in float64. Not inlined: rare, and its registers would
+// be the kernel's.
+template <typename T>
+__device__ __noinline__ double chunk_squares64(const T* v, int vecs) {
+  constexpr int E = 16 / sizeof(T);
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < vecs; k += kThreads)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum = fma((double)to_f(v[k * E + e]), (double)to_f(v[k * E + e]), sum);
+  return sum;
+}
+
 template <typename T, bool MAX>
 __device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t chunk, uint32_t chunks, Acc<MAX>& acc) {
-  using S = Span<T>;
+  using S = Span<T, kNormVecs>;
+  using V = Vec<T, S::E>;
   const S sp(p, count, chunk);
-  const uint4* v = reinterpret_cast<const uint4*>(p + sp.head);
-  uint4 raw[4];
+  const T* body = p + sp.head + sp.v0 * S::E;
+  const V* v = reinterpret_cast<const V*>(body) + threadIdx.x;
+  V raw[kNormVecs];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
-    raw[i] = k < sp.v1 ? v[k] : make_uint4(0, 0, 0, 0);
-  }
+  for (int i = 0; i < kNormVecs; ++i) {
+    if (i * kThreads + (int)threadIdx.x < sp.vecs) {
+      raw[i] = v[i * kThreads];
+    } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (sp.v0 + i * kThreads + threadIdx.x >= sp.v1) break;
-    const T* e = reinterpret_cast<const T*>(&raw[i]);
-    float f[S::E];
-#pragma unroll
-    for (int j = 0; j < S::E; ++j) f[j] = elem(e[j]);
-    acc.template add<S::E>(f);
-  }
-  if (chunk == 0 && (int64_t)threadIdx.x < sp.head) {
-    const float f = elem(p[threadIdx.x]);
-    acc.template add<1>(&f);
-  }
-  if (chunk == chunks - 1) {
-    const int64_t k = sp.head + sp.body * S::E + threadIdx.x;
-    if (k < count) {
-      const float f = elem(p[k]);
-      acc.template add<1>(&f);
+      for (int e = 0; e < S::E; ++e) raw[i].v[e] = from_f<T>(0.f);
     }
   }
+  if constexpr (MAX) {
+#pragma unroll
+    for (int i = 0; i < kNormVecs; ++i)
+#pragma unroll
+      for (int e = 0; e < S::E; ++e) acc.add(to_f(raw[i].v[e]));
+  } else {
+    // A vector's squares in float32 (8 terms of one sign), the vectors in float64, as long as
+    // every vector's sum lies between 2^-100 and 2^126 (none of its terms of weight is below the
+    // normal numbers then) or the vector is all zeros.
+    double sum = 0.0;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < kNormVecs; ++i) {
+      F2 s = f2(0.f);
+#pragma unroll
+      for (int e = 0; e < S::E; e += 2) {
+        const F2 f = unpack(raw[i].v + e);
+        s = fma2(f, f, s);
+      }
+      const float t = both(s);
+      sum += (double)t;
+      if (!(t >= 0x1p-100f && t <= 0x1p126f)) {
+        uint32_t any = 0;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= w[k] & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu);
+        fine = fine && any == 0;
+      }
+    }
+    acc.sum += fine ? sum : chunk_squares64(body, sp.vecs);
+  }
+  if (chunk == 0 && (int)threadIdx.x < sp.head) acc.add(to_f(p[threadIdx.x]));
+  if (chunk == chunks - 1 && sp.tail + threadIdx.x < count) acc.add(to_f(p[sp.tail + threadIdx.x]));
 }
 
 // The block's total of `acc` in thread 0 (as a double: the sum, or the magnitude's bits).
@@ -181,12 +197,13 @@ __device__ __forceinline__ float join_partials(const double* part, int slots) {
 }
 
 template <int N, bool MAX>
-__global__ void __launch_bounds__(kThreads) k_grad_norm(const __grid_constant__ Table<N> t, double* part) {
+__global__ void __launch_bounds__(kThreads, kNormBlocks) k_grad_norm(const __grid_constant__ Table<N> t, double* part) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
   Acc<MAX> acc;
   const uint32_t all = t.first[t.n];
+  int i = 0;
   for (uint32_t c = blockIdx.x; c < all; c += gridDim.x) {
-    const int i = find_tensor(t, c);
+    if (c >= t.first[i + 1]) i = find_tensor(t, c, i + 1, t.n);
     const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
     switch (t.kind[i] & 3) {
       case LEWM_TYPE_F32: chunk_norm(static_cast<const float*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
@@ -211,38 +228,48 @@ __global__ void __launch_bounds__(kThreads) k_norm_out(const double* part, int s
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const T* src, T* dst, int64_t count, uint32_t chunk, uint32_t chunks,
                                             bool single, float coef) {
-  using S = Span<T>;
+  using S = Span<T, kScaleVecs>;
+  using V = Vec<T, S::E>;
   if (single) {
     // src and dst lie differently to 16-byte boundaries: element by element, in chunks of as
     // many elements as vectors would move.
-    const int64_t e0 = (int64_t)chunk * (kChunkBytes / sizeof(T));
-    const int64_t e1 = chunk == chunks - 1 ? count : e0 + kChunkBytes / sizeof(T);
-    for (int64_t k = e0 + threadIdx.x; k < e1; k += kThreads) put(dst + k, elem(src[k]) * coef);
+    constexpr int64_t n = (int64_t)kThreads * kScaleVecs * S::E;
+    const int64_t e0 = chunk * n, e1 = chunk == chunks - 1 ? count : e0 + n;
+#pragma unroll 4
+    for (int64_t k = e0 + threadIdx.x; k < e1; k += kThreads) dst[k] = from_f<T>(to_f(src[k]) * coef);
     return;
   }
   const S sp(src, count, chunk);
-  const uint4* v = reinterpret_cast<const uint4*>(src + sp.head);
-  uint4* o = reinterpret_cast<uint4*>(dst + sp.head);
-  uint4 raw[4];
+  const V* v = reinterpret_cast<const V*>(src + sp.head) + sp.v0 + threadIdx.x;
+  V* o = reinterpret_cast<V*>(dst + sp.head) + sp.v0 + threadIdx.x;
+  const F2 c = f2(coef);
+  auto scale = [&](V& x) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
-    if (k < sp.v1) raw[i] = v[k];
-  }
+    for (int e = 0; e < S::E; e += 2) pack(x.v + e, unpack(x.v + e) * c);
+  };
+  V raw[kScaleVecs];
+  if (sp.vecs == kThreads * kScaleVecs) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t k = sp.v0 + i * kThreads + threadIdx.x;
-    if (k >= sp.v1) break;
-    T* e = reinterpret_cast<T*>(&raw[i]);
+    for (int i = 0; i < kScaleVecs; ++i) raw[i] = v[i * kThreads];
 #pragma unroll
-    for (int j = 0; j < S::E; ++j) put(e + j, elem(e[j]) * coef);
-    o[k] = raw[i];
+    for (int i = 0; i < kScaleVecs; ++i) {
+      scale(raw[i]);
+      o[i * kThreads] = raw[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kScaleVecs; ++i)
+      if (i * kThreads + (int)threadIdx.x < sp.vecs) raw[i] = v[i * kThreads];
+#pragma unroll
+    for (int i = 0; i < kScaleVecs; ++i)
+      if (i * kThreads + (int)threadIdx.x < sp.vecs) {
+        scale(raw[i]);
+        o[i * kThreads] = raw[i];
+      }
   }
-  if (chunk == 0 && (int64_t)threadIdx.x < sp.head) put(dst + threadIdx.x, elem(src[threadIdx.x]) * coef);
-  if (chunk == chunks - 1) {
-    const int64_t k = sp.head + sp.body * S::E + threadIdx.x;
-    if (k < count) put(dst + k, elem(src[k]) * coef);
-  }
+  if (chunk == 0 && (int)threadIdx.x < sp.head) dst[threadIdx.x] = from_f<T>(to_f(src[threadIdx.x]) * coef);
+  const int64_t k = sp.tail + threadIdx.x;
+  if (chunk == chunks - 1 && k < count) dst[k] = from_f<T>(to_f(src[k]) * coef);
 }
 
 // Factor of the clip; a NaN norm gives NaN, as min(1, NaN) must not hide it.
@@ -252,7 +279,7 @@ __device__ __forceinline__ float clip_factor(float norm, float max_norm) {
 }
 
 template <int N, bool MAX>
-__global__ void __launch_bounds__(kThreads) k_grad_scale(const __grid_constant__ Table<N> t, const double* part,
+__global__ void __launch_bounds__(kThreads, kScaleBlocks) k_grad_scale(const __grid_constant__ Table<N> t, const double* part,
                                                          int slots, const float* norm_in, float max_norm,
                                                          float* norm_out, int in_place) {
   griddep_wait();
@@ -262,9 +289,10 @@ __global__ void __launch_bounds__(kThreads) k_grad_scale(const __grid_constant__
   if (in_place && coef == 1.f) return;  // every element times 1 is itself
   const uint32_t all = t.first[t.n];
   // Last chunks first: they are what the norm left in L2 when the gradients exceed it.
+  int i = t.n - 1;
   for (uint32_t k = blockIdx.x; k < all; k += gridDim.x) {
     const uint32_t c = all - 1 - k;
-    const int i = find_tensor(t, c);
+    if (c < t.first[i]) i = find_tensor(t, c, 0, i);
     const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
     const bool single = t.kind[i] & 4;
     switch (t.kind[i] & 3) {
@@ -332,14 +360,14 @@ lewm_status check_list(const GradList& l, int32_t kind, const void* ws, const vo
 // Fills `t` with the tensors from `from` on that fit; empty ones take no place. Returns the
 // index of the first tensor left.
 template <int N>
-int32_t fill_table(const GradList& l, int32_t from, Table<N>* t) {
+int32_t fill_table(const GradList& l, int32_t from, int chunk_bytes, Table<N>* t) {
   t->n = 0;
   uint64_t chunks = 0;
   int32_t i = from;
   for (; i < l.n && t->n < N; ++i) {
     if (l.counts[i] == 0) continue;
     const int64_t bytes = l.counts[i] * type_bytes(l.types[i]);
-    const uint64_t c = (uint64_t)((bytes + kChunkBytes - 1) / kChunkBytes);
+    const uint64_t c = (uint64_t)((bytes + chunk_bytes - 1) / chunk_bytes);
     if (chunks + c > 0xfffffff0ull) break;
     const int k = t->n++;
     t->src[k] = l.src[i];
@@ -359,11 +387,11 @@ cudaError_t run_norm(const GradList& l, double* part, int* slots, cudaStream_t s
   Table<N> t;
   *slots = 0;
   for (int32_t i = 0; i < l.n;) {
-    i = fill_table(l, i, &t);
+    i = fill_table(l, i, kThreads * kNormVecs * 16, &t);
     if (t.n == 0) continue;
     const int32_t launches_left = (l.n - i + N - 1) / N;  // each gets its share of the slots
     const int room = (kSlots - *slots) / (launches_left + 1);
-    const int grid = (int)std::min<uint32_t>(t.first[t.n], (uint32_t)std::min(kBlocks, room));
+    const int grid = (int)std::min<uint32_t>(t.first[t.n], (uint32_t)std::min(kSms * kNormBlocks, room));
     const cudaError_t e = launch_k(k_grad_norm<N, MAX>, dim3(grid), dim3(kThreads), 0, st, t, part + *slots);
     if (e != cudaSuccess) return e;
     *slots += grid;
@@ -377,10 +405,10 @@ cudaError_t run_scale(const GradList& l, const double* part, int slots, const fl
   Table<N> t;
   int32_t i = 0;
   do {
-    i = fill_table(l, i, &t);
+    i = fill_table(l, i, kThreads * kScaleVecs * 16, &t);
     int in_place = 1;
     for (int k = 0; k < t.n; ++k) in_place &= t.src[k] == t.dst[k];
-    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(t.first[t.n], (uint32_t)kBlocks));
+    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(t.first[t.n], (uint32_t)(kSms * kScaleBlocks)));
     const cudaError_t e = launch_k(k_grad_scale<N, MAX>, dim3(grid), dim3(kThreads), 0, st, t, part, slots, norm_in,
                                    max_norm, norm_out, in_place);
     if (e != cudaSuccess) return e;
@@ -420,13 +448,14 @@ lewm_status grad_call(const GradList& l, int32_t kind, float max_norm, const flo
   if (cd.err != cudaSuccess)
     return clip_fail(LEWM_CUDA_ERROR, "cudaSetDevice(%d): %s", device, cudaGetErrorString(cd.err));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool mx = kind == LEWM_NORM_MAX;
-  // A short list takes the small table: parameters are copied on every launch.
-  const cudaError_t e =
-      l.n <= kSmall ? (mx ? run_all<kSmall, true>(l, max_norm, norm_in, ws, norm_out, st)
-                          : run_all<kSmall, false>(l, max_norm, norm_in, ws, norm_out, st))
-                    : (mx ? run_all<kLarge, true>(l, max_norm, norm_in, ws, norm_out, st)
-                          : run_all<kLarge, false>(l, max_norm, norm_in, ws, norm_out, st));
+  // The smallest table that holds the list: the parameters are copied on every launch.
+  auto run = [&](auto max) {
+    constexpr bool MAX = decltype(max)::value;
+    if (l.n <= kSmall) return run_all<kSmall, MAX>(l, max_norm, norm_in, ws, norm_out, st);
+    if (l.n <= kMiddle) return run_all<kMiddle, MAX>(l, max_norm, norm_in, ws, norm_out, st);
+    return run_all<kLarge, MAX>(l, max_norm, norm_in, ws, norm_out, st);
+  };
+  const cudaError_t e = kind == LEWM_NORM_MAX ? run(std::true_type{}) : run(std::false_type{});
   if (e != cudaSuccess) return clip_fail(LEWM_CUDA_ERROR, "gradient norm launch: %s", cudaGetErrorString(e));
   return LEWM_OK;
 }
