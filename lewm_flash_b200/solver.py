@@ -43,6 +43,7 @@ import numpy as np
 import torch
 
 from .runtime import PlanOptions, Runtime
+from .training import clip_grad_norm_
 
 COLORED_NOISE_BETA = {"none": 0.0, "pink": 1.0, "brown": 2.0}
 
@@ -570,6 +571,11 @@ class B200CEMGDSolver(B200ICEMSolver):
     of ``batch_size`` as the reference does (its loss is the mean over a batch's seeds, which
     Adam's epsilon sees). The gradient step's forward and reverse pass are one device call:
     ``gd_forward_time_ms_mean`` times it, ``gd_backward_time_ms_mean`` is 0.
+
+    ``gd_max_grad_norm`` (not in the reference; None: off) clips the gradient of a batch's seeds,
+    taken as one vector, to that norm before Adam steps on it (``clip_grad_norm_``): a seed in a
+    steep place then does not blow up Adam's second moments for the steps after. The summary's
+    gradient norms are those before the clip.
     """
 
     def __init__(self, model: Any | None = None, batch_size: int = 1, num_samples: int = 300, var_scale: float = 1.0,
@@ -579,7 +585,7 @@ class B200CEMGDSolver(B200ICEMSolver):
                  return_best_elite: bool = False, clip_actions: bool = False, gd_seed_solver: str = "cem",
                  gd_seed_source: str = "best_elite", gd_refine_topk: int = 1, gd_steps: int = 1, gd_lr: float = 0.01,
                  gd_compile_cost: bool = False, gd_backtracking: bool = True, callbacks: list[Any] | None = None,
-                 history_size: int = 3) -> None:
+                 history_size: int = 3, gd_max_grad_norm: float | None = None) -> None:
         if topk <= 0:
             raise ValueError(f"topk must be positive, got {topk}")
         if num_samples < topk:
@@ -609,6 +615,8 @@ class B200CEMGDSolver(B200ICEMSolver):
             raise ValueError(f"gd_steps must be non-negative, got {gd_steps}")
         if gd_lr <= 0.0:
             raise ValueError(f"gd_lr must be positive, got {gd_lr}")
+        if gd_max_grad_norm is not None and not gd_max_grad_norm > 0.0:
+            raise ValueError(f"gd_max_grad_norm must be positive, got {gd_max_grad_norm}")
         super().__init__(model, batch_size=batch_size, num_samples=num_samples, var_scale=var_scale, n_steps=n_steps,
                          topk=topk, device=device, seed=seed, elite_retention=elite_retention,
                          colored_noise=colored_noise, colored_noise_time=colored_noise_time,
@@ -622,6 +630,7 @@ class B200CEMGDSolver(B200ICEMSolver):
         self.gd_lr = float(gd_lr)
         self.gd_compile_cost = bool(gd_compile_cost)
         self.gd_backtracking = bool(gd_backtracking)
+        self.gd_max_grad_norm = None if gd_max_grad_norm is None else float(gd_max_grad_norm)
 
     def configure(self, *, action_space: Any, n_envs: int, config: Any) -> None:
         """``CEMGDSolver.configure`` (``cem_gd.py:134-157``): no callback protocol."""
@@ -708,6 +717,8 @@ class B200CEMGDSolver(B200ICEMSolver):
             grad_norms = params.grad.detach().flatten(start_dim=2).norm(dim=2)
             grad_norm_values.extend(grad_norms.cpu().flatten().tolist())
             grad_norm_max = max(grad_norm_max, float(grad_norms.max().item()))
+            if self.gd_max_grad_norm is not None:
+                clip_grad_norm_(params, self.gd_max_grad_norm)
             before = params.detach().clone()
             previous_costs = current_costs.detach().clone()
             optimizer.step()

@@ -532,3 +532,48 @@ def test_training_step_of_a_predictor_with_installed_norms(mode):
         assert not clone(x, c).any() and model(x, c).any()
     handle.remove()
     assert all("forward" not in m.__dict__ for m in model.modules())
+
+
+def test_cem_gd_steps_on_the_clipped_gradient():
+    """_refine_seed_actions with gd_max_grad_norm against Adam on the device gradient clipped by hand in
+    float64 (without backtracking every Adam step is a candidate). The two gradients differ by float32
+    roundings of the factor, 4 u relative; Adam's update m / sqrt(v) is homogeneous of degree 0 in a common
+    scale and moves by lr times such a relative change, so actions agree to 1e-5 lr x steps; the
+    threshold is low enough that the unclipped run ends elsewhere (steps of unlike size then weigh
+    alike in Adam's moments)."""
+    desc = lf.ModelDesc()
+    rt = lf.Runtime(desc, lf.synthetic_state_dict(desc, 3), DEV, model_cost_autocast="none")
+    emb, goal = randn(2, 1, desc.dim, seed=1), randn(2, 1, desc.dim, seed=2)
+    seeds = randn(2, 4, 5, desc.action_dim, seed=3, scale=2.0)
+    costs = rt.model_cost(emb, goal, seeds)
+    lr, steps = 0.5, 4
+
+    def refine(limit):
+        solver = lf.B200CEMGDSolver(model=rt, batch_size=2, topk=4, num_samples=8, gd_refine_topk=4, gd_steps=steps,
+                                    gd_lr=lr, gd_backtracking=False, device=DEV, gd_max_grad_norm=limit)
+        return solver._refine_seed_actions(seeds, costs, emb, goal)[0]
+
+    def by_hand(limit):
+        p = seeds.clone().requires_grad_(True)
+        opt = torch.optim.Adam([p], lr=lr)
+        w = torch.full((2, 4), 1.0 / 8, device=DEV)
+        best, best_costs = seeds.clone(), costs.clone()
+        for _ in range(steps):
+            _, g = rt.model_cost_grad(emb, goal, p.detach(), cost_weights=w)
+            p.grad = (g.double() * min(1.0, limit / (float(g.double().norm()) + 1e-6))).float()
+            before = p.detach().clone()
+            opt.step()
+            c = rt.model_cost(emb, goal, p.detach())
+            better = c < best_costs
+            best = torch.where(better[..., None, None], p.detach(), before)
+            best_costs = torch.where(better, c, best_costs)
+            with torch.no_grad():
+                p.copy_(best)
+        return torch.where((best_costs < costs)[..., None, None], best, seeds)
+
+    _, g0 = rt.model_cost_grad(emb, goal, seeds, cost_weights=torch.full((2, 4), 1.0 / 8, device=DEV))
+    limit = 0.3 * float(g0.norm())
+    got = refine(limit)
+    rt.sync()
+    assert (got - by_hand(limit)).abs().max() <= 1e-5 * lr * steps
+    assert torch.equal(refine(None), refine(math.inf)) and not torch.equal(got, refine(None))

@@ -229,3 +229,10 @@ def test_install_leaves_other_modules_alone():
     model = torch.nn.Sequential(torch.nn.LayerNorm((3, 8)), torch.nn.Linear(8, 8), torch.nn.BatchNorm1d(8),
                                 torch.nn.LayerNorm(8))
     assert lf.install_training_norms(model).modules == ["3"]
+
+
+@pytest.mark.parametrize("value", [0.0, -1.0, math.nan])
+def test_cem_gd_gradient_clip_must_be_positive(value):
+    with pytest.raises(ValueError, match="gd_max_grad_norm must be positive"):
+        lf.B200CEMGDSolver(model=None, gd_max_grad_norm=value)
+    assert lf.B200CEMGDSolver(model=None).gd_max_grad_norm is None
