@@ -308,23 +308,27 @@ struct Stage {
         }
       }
     } else {
-      const uintptr_t s = reinterpret_cast<uintptr_t>(row), e = s + (uintptr_t)width * sizeof(P);
-      const uintptr_t origin = s & ~(uintptr_t)15;  // lies at the slot's start
-      const uint32_t slot = buf + Tm::team() * SLOT;
-      const uintptr_t a0 = (s + 15) & ~(uintptr_t)15, last = e & ~(uintptr_t)15, a1 = last > a0 ? last : a0;
-      for (uintptr_t a = a0 + 16 * lane; a < a1; a += 16 * TPR)
-        cp_async16(slot + (uint32_t)(a - origin), reinterpret_cast<const void*>(a));
-      if (lane < 8) {  // up to four 4-byte words before a0 and after a1
-        const uintptr_t w = lane < 4 ? (s & ~(uintptr_t)3) + 4 * lane : a1 + 4 * (lane - 4);
-        if (w < (lane < 4 ? (a0 < e ? a0 : e) : e)) {
-          if (w >= reinterpret_cast<uintptr_t>(lo) && w + 4 <= reinterpret_cast<uintptr_t>(hi)) {
-            cp_async4(slot + (uint32_t)(w - origin), reinterpret_cast<const void*>(w));
+      // Byte offsets from the row's start, which lies `mis` bytes behind the slot's: 16-byte pieces
+      // [a0, a1), up to four 4-byte words before and after them.
+      const int mis = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = width * (int)sizeof(P);
+      const int a0 = (16 - mis) & 15, a1 = max(a0, ((mis + bytes) & ~15) - mis);
+      const uint32_t slot = buf + Tm::team() * SLOT + mis;
+      const char* src = reinterpret_cast<const char*>(row);
+      constexpr int PIECES = (NV * (int)sizeof(P) + 15) / 16;  // of a thread at most
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        const int a = a0 + 16 * (lane + k * TPR);
+        if (a < a1) cp_async16(slot + a, src + a);
+      }
+      if (lane < 8) {
+        const int w = lane < 4 ? -(mis & 3) + 4 * lane : a1 + 4 * (lane - 4);
+        if (w < (lane < 4 ? min(a0, bytes) : bytes)) {
+          if (src + w >= reinterpret_cast<const char*>(lo) && src + w + 4 <= reinterpret_cast<const char*>(hi)) {
+            cp_async4(slot + w, src + w);
           } else {
-            for (uintptr_t q = w; q < w + 4; q += sizeof(P))
-              if (q >= s && q < e) {
-                P* d = reinterpret_cast<P*>(__cvta_shared_to_generic(slot + (uint32_t)(q - origin)));
-                *d = *reinterpret_cast<const P*>(q);
-              }
+            for (int q = w; q < w + 4; q += (int)sizeof(P))
+              if (q >= 0 && q < bytes)
+                *reinterpret_cast<P*>(__cvta_shared_to_generic(slot + q)) = *reinterpret_cast<const P*>(src + q);
           }
         }
       }
@@ -413,16 +417,34 @@ struct Walk {
         step(step_rows * stride) {}
 };
 
-// Blocks per SM that the registers are limited for: 80 a thread forward, 128 in the backward that
-// keeps sums. More, smaller blocks were slower on short rows (16448 x 192 bf16 forward, 3, 4 and 5
+// Blocks per SM that the registers are limited for: 80 a thread forward (128 with 32 values), 128 in
+// the backward that keeps sums. More, smaller blocks were slower on short rows (16448 x 192 bf16 forward, 3, 4 and 5
 // blocks: 6.8, 6.9, 7.2 us): every block loads the parameters anew. The backward of a modulation
 // row per row has neither and takes 4 there (57600 x 192 bf16, 2, 3 and 4 blocks: 26.2, 22.9,
 // 21.6 us).
 template <typename Tm>
 constexpr int bound_blocks(bool backward, bool rowmod = false) {
   if (rowmod && backward && Tm::N == 8) return 4;
-  const int n = (backward ? 512 : 768) / Tm::THREADS;
+  const int n = (backward || Tm::N == 32 ? 512 : 768) / Tm::THREADS;
   return n > 0 ? n : 1;
+}
+
+// What multiplies z in group g, and what is added: weight or 1 + scale, bias or shift.
+template <typename Tm>
+__device__ __forceinline__ void load_gain(const NormArgs& p, int64_t g, F2* a) {
+#pragma unroll
+  for (int k = 0; k < Tm::H; ++k) a[k] = f2(p.one_plus ? 0.f : 1.f);
+  if (p.a) Tm::load_params(p.a, p.p_type, g * p.a_stride, p.width, p.p_vec, a);
+  if (p.one_plus) {
+#pragma unroll
+    for (int k = 0; k < Tm::H; ++k) a[k] = a[k] + f2(1.f);
+  }
+}
+template <typename Tm>
+__device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b) {
+#pragma unroll
+  for (int k = 0; k < Tm::H; ++k) b[k] = f2(0.f);
+  if (p.b) Tm::load_params(p.b, p.p_type, g * p.b_stride, p.width, p.p_vec, b);
 }
 
 // ------------------------------------------------------------------ forward
@@ -481,15 +503,9 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_norm_f
     };
     for (int k = 0; k < p.stages - 1; ++k) fetch();
     F2 ga[H], gb[H];
-#pragma unroll
-    for (int k = 0; k < H; ++k) ga[k] = f2(p.one_plus ? 0.f : 1.f), gb[k] = f2(0.f);
     if (left > 0) {
-      if (p.a) Tm::load_params(p.a, p.p_type, it.g * p.a_stride, p.width, p.p_vec, ga);
-      if (p.b) Tm::load_params(p.b, p.p_type, it.g * p.b_stride, p.width, p.p_vec, gb);
-    }
-    if (p.one_plus) {
-#pragma unroll
-      for (int k = 0; k < H; ++k) ga[k] = ga[k] + f2(1.f);
+      load_gain<Tm>(p, it.g, ga);
+      load_offset<Tm>(p, it.g, gb);
     }
     int64_t r = it.first;
     T* y = static_cast<T*>(p.out) + r * p.width;
@@ -641,12 +657,8 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true)) k_norm_bw
     for (int k = 0; k < p.stages - 1; ++k) fetch();
     F2 ga[H], sa[H], sb[H];
 #pragma unroll
-    for (int k = 0; k < H; ++k) ga[k] = f2(p.one_plus ? 0.f : 1.f), sa[k] = sb[k] = f2(0.f);
-    if (p.a && any) Tm::load_params(p.a, p.p_type, it.g * p.a_stride, p.width, p.p_vec, ga);
-    if (p.one_plus) {
-#pragma unroll
-      for (int k = 0; k < H; ++k) ga[k] = ga[k] + f2(1.f);
-    }
+    for (int k = 0; k < H; ++k) sa[k] = sb[k] = f2(0.f);
+    if (any) load_gain<Tm>(p, it.g, ga);
     // Statistics of the first row; each row loads the next one's.
     const float* stat = p.stats + it.first;
     float mu = 0.f, rs = 0.f;
@@ -972,27 +984,30 @@ __global__ void __launch_bounds__(256) k_norm_sums_wide(const NormArgs p) {
 }
 
 // ------------------------------------------------------------------ host side
-// Team size of a row: threads x elements per thread covers the width.
+// Team of a row: threads x elements per thread covers the width.
 struct Tier {
-  int tpr, teams, ept;
+  int tpr, ept;
+  int teams() const { return block_threads(tpr) / tpr; }
 };
-Tier tier_of(int64_t width) {
-  if (width <= 64) return {8, 32, 8};
-  if (width <= 256) return {32, 8, 8};
+Tier tier_of(int64_t width, bool backward) {
+  if (width <= 64) return {8, 8};
+  if (width <= 256) return {32, 8};
+  // The forward keeps no sums: 32 values a thread leave two blocks per SM where 16 leave one.
+  if (!backward && width > 4096 && width <= 8192) return {256, 32};
   int tpr = 32;
   while (tpr * 16 < width) tpr *= 2;  // rows of at most kMaxRowBytes: tpr <= 1024
-  return {tpr, block_threads(tpr) / tpr, 16};
+  return {tpr, 16};
 }
 int64_t type_size(int type) { return type == LEWM_TYPE_F32 ? 4 : 2; }
 bool is_wide(const NormArgs& p, int x_type) { return p.width * type_size(x_type) > kMaxRowBytes; }
 
 // Blocks that fill the GPU once.
 int64_t full_grid(const Tier& t, bool backward) {
-  return (int64_t)kSms * (t.tpr <= 256   ? bound_blocks<Team<1, 16, 32>>(backward)
-                          : t.tpr == 512 ? bound_blocks<Team<1, 16, 512>>(backward)
-                                         : bound_blocks<Team<1, 16, 1024>>(backward));
+  return (int64_t)kSms * (t.ept == 32      ? bound_blocks<Team<1, 32, 256>>(backward)
+                          : t.tpr <= 256   ? bound_blocks<Team<1, 16, 256>>(backward)
+                          : t.tpr == 512   ? bound_blocks<Team<1, 16, 512>>(backward)
+                                           : bound_blocks<Team<1, 16, 1024>>(backward));
 }
-
 // Rounds of loops over `rows` rows in steps of `step`. (No tensor that fits a GPU makes 2^31 rounds: a
 // step is a row for groups of a few, else a block's teams times the blocks that share the rows.)
 void set_loop(NormArgs* p, int64_t rows, int64_t step) {
@@ -1010,16 +1025,16 @@ void cut_items(NormArgs* p, int x_type, bool backward) {
     p->team_items = 0;
     p->split = (int)std::max<int64_t>(1, std::min<int64_t>(want, p->group));
   } else {
-    const Tier t = tier_of(p->width);
+    const Tier t = tier_of(p->width, backward);
     // A team's items where a group has too few rows to keep a block's teams busy and there
     // are groups enough to fill the GPU without splitting them.
-    p->team_items = p->group < 2 * t.teams && groups >= 2 * kSms;
+    p->team_items = p->group < 2 * t.teams() && groups >= 2 * kSms;
     const int64_t want = full_grid(t, backward) / groups;  // one wave of blocks
-    const int64_t most = (p->group + t.teams - 1) / t.teams;
+    const int64_t most = (p->group + t.teams() - 1) / t.teams();
     p->split = p->team_items ? 1 : (int)std::max<int64_t>(1, std::min(want, most));
   }
   p->items = groups * p->split;
-  set_loop(p, p->group, p->team_items ? 1 : (int64_t)p->split * (is_wide(*p, x_type) ? 1 : tier_of(p->width).teams));
+  set_loop(p, p->group, p->team_items ? 1 : (int64_t)p->split * (is_wide(*p, x_type) ? 1 : tier_of(p->width, backward).teams()));
 }
 
 size_t workspace_bytes(const NormArgs& p) {
@@ -1052,6 +1067,12 @@ cudaError_t launch_ring(K kern, bool* raised, int64_t grid, int threads, int sme
   return launch_k(kern, dim3((unsigned)grid), dim3(threads), smem, st, p);
 }
 
+// The passes that use a tier (tier_of).
+template <typename Tm>
+constexpr bool has_backward = Tm::N != 32;
+template <typename Tm>
+constexpr bool has_forward = !(Tm::N == 16 && Tm::TPR == 512);
+
 template <typename T, typename Tm>
 cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
   static bool raised[2][64];  // only ever set to true: calls from several threads may repeat the attribute
@@ -1059,8 +1080,11 @@ cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
   p.stages = ring_stages(bytes, bound_blocks<Tm>(backward));
   const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
   const int64_t grid = std::min(blocks, (int64_t)kSms * bound_blocks<Tm>(backward));
-  return backward ? launch_ring(k_norm_bwd<T, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
-                  : launch_ring(k_norm_fwd<T, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
+  if constexpr (has_backward<Tm>)
+    if (backward) return launch_ring(k_norm_bwd<T, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st);
+  if constexpr (has_forward<Tm>)
+    if (!backward) return launch_ring(k_norm_fwd<T, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
+  return cudaErrorInvalidValue;  // not a tier of this pass
 }
 
 // group 1: the modulation in the ring, if two stages of it fit.
@@ -1073,8 +1097,11 @@ cudaError_t launch_rowmod(NormArgs p, bool backward, cudaStream_t st) {
   if (p.stages == 0) return launch_items<T, Tm>(p, backward, st);
   const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, (int64_t)kSms * bound_blocks<Tm>(backward, true));
   set_loop(&p, p.rows, grid * Tm::TEAMS);
-  return backward ? launch_ring(k_rowmod_bwd<T, P, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st)
-                  : launch_ring(k_rowmod_fwd<T, P, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
+  if constexpr (has_backward<Tm>)
+    if (backward) return launch_ring(k_rowmod_bwd<T, P, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st);
+  if constexpr (has_forward<Tm>)
+    if (!backward) return launch_ring(k_rowmod_fwd<T, P, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
+  return cudaErrorInvalidValue;  // not a tier of this pass
 }
 
 template <typename T, int E, int NV, int TPR>
@@ -1092,11 +1119,12 @@ cudaError_t launch_tier(const NormArgs& p, bool backward, cudaStream_t st) {
 
 template <typename T, int E>
 cudaError_t launch_width(const NormArgs& p, bool backward, cudaStream_t st) {
-  constexpr int V8 = 8 / E, V16 = 16 / E;
-  switch (tier_of(p.width).tpr) {
-    case 8: return launch_tier<T, E, V8, 8>(p, backward, st);
-    case 32:
-      return p.width <= 256 ? launch_tier<T, E, V8, 32>(p, backward, st) : launch_tier<T, E, V16, 32>(p, backward, st);
+  constexpr int V8 = 8 / E, V16 = 16 / E, V32 = 32 / E;
+  const Tier t = tier_of(p.width, backward);
+  if (t.ept == 8) return t.tpr == 8 ? launch_tier<T, E, V8, 8>(p, backward, st) : launch_tier<T, E, V8, 32>(p, backward, st);
+  if (t.ept == 32) return launch_tier<T, E, V32, 256>(p, false, st);
+  switch (t.tpr) {
+    case 32: return launch_tier<T, E, V16, 32>(p, backward, st);
     case 64: return launch_tier<T, E, V16, 64>(p, backward, st);
     case 128: return launch_tier<T, E, V16, 128>(p, backward, st);
     case 256: return launch_tier<T, E, V16, 256>(p, backward, st);
