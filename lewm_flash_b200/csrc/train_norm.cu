@@ -1041,13 +1041,19 @@ size_t workspace_bytes(const NormArgs& p) {
   return p.split > 1 ? (size_t)p.items * 2 * (size_t)p.width * sizeof(float) : 0;
 }
 
-// Stages of `bytes` each that fit `blocks` blocks per SM, 4 at most; 0 where not even two fit one
-// block.
+// Stages of `bytes` each for `blocks` blocks per SM (fewer if they do not fit): 2 to 4, as many as
+// keep `ahead` bytes per SM on their way; 0 where not even two fit one block. More than needed is
+// slower: rows fetched far ahead compete with the stores in DRAM. 48 KB do where a pass writes as
+// much as it reads (73881 x 1536 float32 forward with 2, 3 and 4 stages of 48 KB per SM: 142, 170
+// and 172 us; 131072 x 2048 bf16 with 24 KB stages: 184, 174, 183), 96 KB in the backward (float32
+// with 64 KB stages: 209, 203, 203; bf16 with 32 KB: 276, 258, 260).
 constexpr int kSmemPerSm = 227 * 1024, kSmemReserved = 2 * 1024;  // the latter: static and the system's, per block
-int ring_stages(int bytes, int blocks) {
+constexpr int kAhead = 48 * 1024, kAheadBackward = 96 * 1024;
+int ring_stages(int bytes, int blocks, int ahead) {
   for (; blocks >= 1; blocks = blocks / 2) {
-    const int n = (kSmemPerSm / blocks - kSmemReserved) / bytes;
-    if (n >= 3 || (blocks == 1 && n >= 2)) return std::min(n, 4);
+    const int fit = (kSmemPerSm / blocks - kSmemReserved) / bytes;
+    const int want = std::min(4, 1 + (ahead + bytes * blocks - 1) / (bytes * blocks));
+    if (fit >= std::min(want, 3) || (blocks == 1 && fit >= 2)) return std::min(fit, std::max(want, 2));
   }
   return 0;
 }
@@ -1077,7 +1083,7 @@ template <typename T, typename Tm>
 cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
   static bool raised[2][64];  // only ever set to true: calls from several threads may repeat the attribute
   const int bytes = (backward ? 2 : 1) * Stage<T, Tm>::BYTES;
-  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward));
+  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward), backward ? kAheadBackward : kAhead);
   const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
   const int64_t grid = std::min(blocks, (int64_t)kSms * bound_blocks<Tm>(backward));
   if constexpr (has_backward<Tm>)
@@ -1093,7 +1099,7 @@ cudaError_t launch_rowmod(NormArgs p, bool backward, cudaStream_t st) {
   static bool raised[2][64];
   const int x_bytes = Stage<T, Tm>::BYTES, p_bytes = Stage<P, Tm>::BYTES;
   const int bytes = backward ? 2 * x_bytes + p_bytes : x_bytes + 2 * p_bytes;
-  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward, true));
+  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward, true), kAhead);
   if (p.stages == 0) return launch_items<T, Tm>(p, backward, st);
   const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, (int64_t)kSms * bound_blocks<Tm>(backward, true));
   set_loop(&p, p.rows, grid * Tm::TEAMS);
