@@ -37,10 +37,12 @@ constexpr int kThreads = 256;
 constexpr int kSms = 148;      // B200
 constexpr int kSlots = 2048;   // partial sums of all launches of a call
 // 16-byte vectors of a chunk per thread, all in flight at once, and blocks per SM. Norm of 2^28 bf16
-// elements with 8 x 4: 82 us (6.5 TB/s), 4 x 8: 101, 4 x 6: 94; norm and scaling with 4 x 4 for the
-// scaling: 275 us, 2 x 8: 290, 4 x 6: 297.
+// elements with 8 x 4: 82 us (6.5 TB/s), 4 x 8: 101, 4 x 6: 94. Norm and scaling with 4 x 3 for the
+// scaling: 265 us, 4 x 4: 274, 2 x 4: 290 (reads on their way compete with the stores in DRAM); of
+// 33.5M mixed elements, half of them still in L2: 4 x 4 52 us, 4 x 3 54.
 constexpr int kNormVecs = 8, kNormBlocks = 4;
-constexpr int kScaleVecs = 4, kScaleBlocks = 4;
+constexpr int kScaleVecs = 4, kScaleBlocks = 4, kScaleBlocksDram = 3;
+constexpr int64_t kL2Bytes = 126 << 20;
 static_assert(kSms * kNormBlocks <= kSlots && kSlots * sizeof(double) <= LEWM_GRAD_WORKSPACE, "workspace");
 
 // A launch's tensors. Element types and whether a tensor's vectors can be 16 bytes (src and
@@ -113,16 +115,16 @@ __device__ __noinline__ double chunk_squares64(const T* v, int vecs) {
   return sum;
 }
 
-template <typename T, bool MAX>
+template <int VECS, typename T, bool MAX>
 __device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t chunk, uint32_t chunks, Acc<MAX>& acc) {
-  using S = Span<T, kNormVecs>;
+  using S = Span<T, VECS>;
   using V = Vec<T, S::E>;
   const S sp(p, count, chunk);
   const T* body = p + sp.head + sp.v0 * S::E;
   const V* v = reinterpret_cast<const V*>(body) + threadIdx.x;
-  V raw[kNormVecs];
+  V raw[VECS];
 #pragma unroll
-  for (int i = 0; i < kNormVecs; ++i) {
+  for (int i = 0; i < VECS; ++i) {
     if (i * kThreads + (int)threadIdx.x < sp.vecs) {
       raw[i] = v[i * kThreads];
     } else {
@@ -132,7 +134,7 @@ __device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t c
   }
   if constexpr (MAX) {
 #pragma unroll
-    for (int i = 0; i < kNormVecs; ++i)
+    for (int i = 0; i < VECS; ++i)
 #pragma unroll
       for (int e = 0; e < S::E; ++e) acc.add(to_f(raw[i].v[e]));
   } else {
@@ -142,7 +144,7 @@ __device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t c
     double sum = 0.0;
     bool fine = true;
 #pragma unroll
-    for (int i = 0; i < kNormVecs; ++i) {
+    for (int i = 0; i < VECS; ++i) {
       F2 s = f2(0.f);
 #pragma unroll
       for (int e = 0; e < S::E; e += 2) {
@@ -165,6 +167,18 @@ __device__ __forceinline__ void chunk_norm(const T* p, int64_t count, uint32_t c
   if (chunk == chunks - 1 && sp.tail + threadIdx.x < count) acc.add(to_f(p[sp.tail + threadIdx.x]));
 }
 
+template <int VECS, int N, bool MAX>
+__device__ __forceinline__ void table_norm(const Table<N>& t, int i, uint32_t c, Acc<MAX>& acc) {
+  const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
+  switch (t.kind[i] & 3) {
+    case LEWM_TYPE_F32: chunk_norm<VECS>(static_cast<const float*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
+    case LEWM_TYPE_BF16:
+      chunk_norm<VECS>(static_cast<const __nv_bfloat16*>(t.src[i]), t.count[i], chunk, chunks, acc);
+      break;
+    default: chunk_norm<VECS>(static_cast<const __half*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
+  }
+}
+
 // The block's total of `acc` in thread 0 (as a double: the sum, or the magnitude's bits).
 template <bool MAX>
 __device__ __forceinline__ double block_total(const Acc<MAX>& acc) {
@@ -184,6 +198,11 @@ __device__ __forceinline__ double block_total(const Acc<MAX>& acc) {
   return v;
 }
 
+template <bool MAX>
+__device__ __forceinline__ float norm_of(double total) {
+  return MAX ? __uint_as_float((uint32_t)total) : (float)sqrt(total);
+}
+
 // Norm of `slots` partials: the same order in every block, so the same bits.
 template <bool MAX>
 __device__ __forceinline__ float join_partials(const double* part, int slots) {
@@ -192,8 +211,7 @@ __device__ __forceinline__ float join_partials(const double* part, int slots) {
     if constexpr (MAX) acc.bits = max(acc.bits, (uint32_t)part[i]);
     else acc.sum += part[i];
   }
-  const double v = block_total<MAX>(acc);
-  return MAX ? __uint_as_float((uint32_t)v) : (float)sqrt(v);
+  return norm_of<MAX>(block_total<MAX>(acc));
 }
 
 template <int N, bool MAX>
@@ -204,14 +222,7 @@ __global__ void __launch_bounds__(kThreads, kNormBlocks) k_grad_norm(const __gri
   int i = 0;
   for (uint32_t c = blockIdx.x; c < all; c += gridDim.x) {
     if (c >= t.first[i + 1]) i = find_tensor(t, c, i + 1, t.n);
-    const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
-    switch (t.kind[i] & 3) {
-      case LEWM_TYPE_F32: chunk_norm(static_cast<const float*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
-      case LEWM_TYPE_BF16:
-        chunk_norm(static_cast<const __nv_bfloat16*>(t.src[i]), t.count[i], chunk, chunks, acc);
-        break;
-      default: chunk_norm(static_cast<const __half*>(t.src[i]), t.count[i], chunk, chunks, acc); break;
-    }
+    table_norm<kNormVecs>(t, i, c, acc);
   }
   const double v = block_total<MAX>(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = v;
@@ -272,6 +283,26 @@ __device__ __forceinline__ void chunk_scale(const T* src, T* dst, int64_t count,
   if (chunk == chunks - 1 && k < count) dst[k] = from_f<T>(to_f(src[k]) * coef);
 }
 
+template <int N>
+__device__ __forceinline__ void table_scale(const Table<N>& t, int i, uint32_t c, float coef) {
+  const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
+  const bool single = t.kind[i] & 4;
+  switch (t.kind[i] & 3) {
+    case LEWM_TYPE_F32:
+      chunk_scale(static_cast<const float*>(t.src[i]), static_cast<float*>(t.dst[i]), t.count[i], chunk, chunks,
+                  single, coef);
+      break;
+    case LEWM_TYPE_BF16:
+      chunk_scale(static_cast<const __nv_bfloat16*>(t.src[i]), static_cast<__nv_bfloat16*>(t.dst[i]), t.count[i],
+                  chunk, chunks, single, coef);
+      break;
+    default:
+      chunk_scale(static_cast<const __half*>(t.src[i]), static_cast<__half*>(t.dst[i]), t.count[i], chunk, chunks,
+                  single, coef);
+      break;
+  }
+}
+
 // Factor of the clip; a NaN norm gives NaN, as min(1, NaN) must not hide it.
 __device__ __forceinline__ float clip_factor(float norm, float max_norm) {
   const float c = max_norm / (norm + 1e-6f);
@@ -293,23 +324,23 @@ __global__ void __launch_bounds__(kThreads, kScaleBlocks) k_grad_scale(const __g
   for (uint32_t k = blockIdx.x; k < all; k += gridDim.x) {
     const uint32_t c = all - 1 - k;
     if (c < t.first[i]) i = find_tensor(t, c, 0, i);
-    const uint32_t chunk = c - t.first[i], chunks = t.first[i + 1] - t.first[i];
-    const bool single = t.kind[i] & 4;
-    switch (t.kind[i] & 3) {
-      case LEWM_TYPE_F32:
-        chunk_scale(static_cast<const float*>(t.src[i]), static_cast<float*>(t.dst[i]), t.count[i], chunk, chunks,
-                    single, coef);
-        break;
-      case LEWM_TYPE_BF16:
-        chunk_scale(static_cast<const __nv_bfloat16*>(t.src[i]), static_cast<__nv_bfloat16*>(t.dst[i]), t.count[i],
-                    chunk, chunks, single, coef);
-        break;
-      default:
-        chunk_scale(static_cast<const __half*>(t.src[i]), static_cast<__half*>(t.dst[i]), t.count[i], chunk, chunks,
-                    single, coef);
-        break;
-    }
+    table_scale(t, i, c, coef);
   }
+}
+
+// A few chunks in one block and one launch: norm, then scaling (dst set).
+template <bool MAX>
+__global__ void __launch_bounds__(kThreads) k_clip_block(const __grid_constant__ Table<kSmall> t, float max_norm,
+                                                         float* norm_out, int scale, int in_place) {
+  griddep_wait();
+  Acc<MAX> acc;
+  const uint32_t all = t.first[t.n];
+  for (uint32_t c = 0; c < all; ++c) table_norm<kScaleVecs>(t, find_tensor(t, c, 0, t.n), c, acc);
+  const float norm = norm_of<MAX>(block_total<MAX>(acc));  // a barrier: all is read before anything is written
+  if (threadIdx.x == 0) *norm_out = norm;
+  const float coef = clip_factor(norm, max_norm);
+  if (!scale || (in_place && coef == 1.f)) return;
+  for (uint32_t c = 0; c < all; ++c) table_scale(t, find_tensor(t, c, 0, t.n), c, coef);
 }
 
 // ------------------------------------------------------------------ host side
@@ -403,12 +434,15 @@ template <int N, bool MAX>
 cudaError_t run_scale(const GradList& l, const double* part, int slots, const float* norm_in, float max_norm,
                       float* norm_out, cudaStream_t st) {
   Table<N> t;
+  int64_t bytes = 0;
+  for (int32_t k = 0; k < l.n; ++k) bytes += l.counts[k] * type_bytes(l.types[k]);
+  const int blocks = kSms * (bytes > kL2Bytes ? kScaleBlocksDram : kScaleBlocks);
   int32_t i = 0;
   do {
     i = fill_table(l, i, kThreads * kScaleVecs * 16, &t);
     int in_place = 1;
     for (int k = 0; k < t.n; ++k) in_place &= t.src[k] == t.dst[k];
-    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(t.first[t.n], (uint32_t)(kSms * kScaleBlocks)));
+    const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(t.first[t.n], (uint32_t)blocks));
     const cudaError_t e = launch_k(k_grad_scale<N, MAX>, dim3(grid), dim3(kThreads), 0, st, t, part, slots, norm_in,
                                    max_norm, norm_out, in_place);
     if (e != cudaSuccess) return e;
@@ -428,6 +462,24 @@ struct ClipDevice {
     if (prev >= 0) cudaSetDevice(prev);
   }
 };
+
+// The whole list in one block, if it is that small: kBlockChunks chunks of the scaling at most (one
+// tensor of 1500 float32: 3.8 us in two launches, 2.2 in one). Returns whether it was launched.
+constexpr uint32_t kBlockChunks = 4;
+template <bool MAX>
+bool run_block(const GradList& l, float max_norm, float* norm_out, cudaStream_t st, cudaError_t* e) {
+  if (l.n > kSmall) return false;
+  int64_t bytes = 0;
+  for (int32_t k = 0; k < l.n; ++k) bytes += l.counts[k] * type_bytes(l.types[k]);
+  if (bytes > (int64_t)kBlockChunks * kThreads * kScaleVecs * 16) return false;
+  Table<kSmall> t;
+  fill_table(l, 0, kThreads * kScaleVecs * 16, &t);
+  if (t.first[t.n] > kBlockChunks) return false;
+  int in_place = 1;
+  for (int k = 0; k < t.n; ++k) in_place &= t.src[k] == t.dst[k];
+  *e = launch_k(k_clip_block<MAX>, dim3(1), dim3(kThreads), 0, st, t, max_norm, norm_out, l.dst ? 1 : 0, in_place);
+  return true;
+}
 
 template <int N, bool MAX>
 cudaError_t run_all(const GradList& l, float max_norm, const float* norm_in, void* ws, float* norm_out,
@@ -451,6 +503,8 @@ lewm_status grad_call(const GradList& l, int32_t kind, float max_norm, const flo
   // The smallest table that holds the list: the parameters are copied on every launch.
   auto run = [&](auto max) {
     constexpr bool MAX = decltype(max)::value;
+    cudaError_t e = cudaSuccess;
+    if (!norm_in && run_block<MAX>(l, max_norm, norm_out, st, &e)) return e;
     if (l.n <= kSmall) return run_all<kSmall, MAX>(l, max_norm, norm_in, ws, norm_out, st);
     if (l.n <= kMiddle) return run_all<kMiddle, MAX>(l, max_norm, norm_in, ws, norm_out, st);
     return run_all<kLarge, MAX>(l, max_norm, norm_in, ws, norm_out, st);
