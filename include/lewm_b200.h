@@ -364,8 +364,10 @@ LEWM_API void lewm_encoder_destroy(lewm_encoder* enc);
  * AdaLN-modulated LayerNorm with their backward passes, and the global gradient norm with
  * clipping. No context: each call works on the given device and stream, allocates nothing,
  * keeps nothing and never synchronizes, so it may be captured into a CUDA graph. Two calls
- * that overlap on the GPU need different workspaces. Results are the same bits on every run
- * of a shape (no atomics). Errors: text from lewm_last_error(NULL). */
+ * that overlap on the GPU need different workspaces. Pointers are aligned to their element type,
+ * and no output overlaps an input or another output except where said. Results are the same bits
+ * on every run of a shape (no atomics). The first call of a kernel loads it onto the device: make
+ * it before a capture. Errors: text from lewm_last_error(NULL). */
 #define LEWM_TYPE_F32 0
 #define LEWM_TYPE_BF16 1
 #define LEWM_TYPE_F16 2

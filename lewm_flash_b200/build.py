@@ -17,8 +17,8 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "liblewm_b200.so"
 SOURCES = ["api.cu", "rollout_kernels.cu", "tile_call.cu", "fp32_path.cu", "icem_kernels.cu", "noalloc.cu", "encoder.cu",
-           "train_norm.cu", "grad_clip.cu"]
-HEADERS = ["lewm_common.cuh", "lewm_internal.h", "train_elem.cuh"]
+           "train_norm.cu", "train_norm_f32.cu", "train_norm_bf16.cu", "train_norm_f16.cu", "grad_clip.cu"]
+HEADERS = ["lewm_common.cuh", "lewm_internal.h", "train_elem.cuh", "train_norm.h", "train_norm.cuh"]
 EXT = PKG / "_torch_ops.so"
 EXT_SOURCES = ["torch_ops.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,8 @@
+// Norm kernels for rows of float.
+#include "train_norm.cuh"
+
+namespace lewm {
+
+template cudaError_t launch_norm_rows<float>(const NormArgs& p, bool wide, bool backward, bool vec, cudaStream_t st);
+
+}  // namespace lewm

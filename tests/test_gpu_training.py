@@ -161,6 +161,24 @@ def test_strided_inputs(make, dtype):
     check_norm(x, w, b, 1e-5, False, 0, y.detach(), dy, dx, dw, db)
 
 
+@pytest.mark.parametrize("dtype,ptype", [(F32, F32), (BF16, F32), (BF16, BF16)], ids=["f32", "bf16-f32", "bf16"])
+@pytest.mark.parametrize("width", [192, 1024, 16640])
+def test_parameters_off_16_bytes(width, dtype, ptype):
+    """Weight, bias, scale and shift that start one element into their allocations."""
+    x = activation(700, width, dtype).requires_grad_(True)
+    w = randn(width + 1, seed=2, scale=0.2, offset=1.0, dtype=ptype)[1:].requires_grad_(True)
+    b = randn(width + 1, seed=3, dtype=ptype)[1:].requires_grad_(True)
+    dy = randn(700, width, seed=4, dtype=dtype)
+    y = lf.layer_norm(x, w, b)
+    check_norm(x, w, b, 1e-5, False, 0, y.detach(), dy, *torch.autograd.grad(y, (x, w, b), dy))
+    for rows, group in ((700, 1), (7, 100)):
+        mod = randn(rows, 2 * width + 3, seed=5, scale=0.3, dtype=ptype)
+        shift, scale = (mod[:, o:o + width].unsqueeze(1).requires_grad_(True) for o in (1, width + 2))
+        y = lf.ada_layer_norm(x.view(rows, group, width), shift, scale)
+        dx, dshift, dscale = torch.autograd.grad(y, (x, shift, scale), dy.view(rows, group, width))
+        check_norm(x, scale, shift, 1e-6, True, group, y.detach(), dy, dx, dscale, dshift)
+
+
 def test_expanded_output_gradient():
     x = randn(33, 192, seed=1).requires_grad_(True)
     w = randn(192, seed=2).requires_grad_(True)

@@ -163,6 +163,17 @@ def test_c_abi_norm_null_pointers_and_workspace():
     assert need > 0 and need % (2 * 8 * 4) == 0
     assert lib.lewm_norm_backward(C.byref(big), P, 8, P, P, P, P, P, None, P, need - 1, 0, None) == 1
     assert "workspace" in lib.lewm_last_error(None).decode()
+    assert lib.lewm_norm_backward(C.byref(big), P, 8, P, P, P, P, P, None, P // 16 * 16 + 8, need, 0, None) == 1
+    assert "aligned" in lib.lewm_last_error(None).decode()
+    # Pointers off their elements.
+    for args in ((P + 2, None, None, P, None), (P, P + 2, None, P, None), (P, None, None, P + 1, None),
+                 (P, None, None, P, P + 2)):
+        assert lib.lewm_norm_forward(C.byref(d), *args, 0, None) == 1
+        assert "not aligned to its element" in lib.lewm_last_error(None).decode()
+    for args in ((P + 2, 8, P, None, P, P, None, None), (P, 8, P + 2, None, P, P, None, None),
+                 (P, 8, P, None, P, P + 2, None, None), (P, 8, P, None, P + 2, P, None, None),
+                 (P, 8, P, None, P, P, P + 2, None), (P, 8, P, None, P, P, None, P + 1)):
+        assert lib.lewm_norm_backward(C.byref(d), *args, None, 0, 0, None) == 1
     # Nothing to do: no rows, or no gradient asked for.
     e = desc(rows=0)
     assert lib.lewm_norm_forward(C.byref(e), None, None, None, None, None, 0, None) == 0
