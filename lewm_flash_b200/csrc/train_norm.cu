@@ -73,32 +73,37 @@ __global__ void __launch_bounds__(256) k_norm_reduce(const NormArgs p) {
 }
 
 // How rows are cut into items; the same function sizes the workspace.
-void cut_items(NormArgs* p, int x_type, bool backward) {
+void cut_items(NormArgs* p, int x_type, bool backward, bool vec) {
   const int64_t groups = p->rows / p->group;
+  int64_t teams = 1;
+  p->team_items = 0;
   if (is_wide(*p, x_type)) {
     // Column blocks x items: split each group until the grid has about 4 blocks per SM.
     const int64_t cols = (p->width + 2047) / 2048;
     const int64_t want = (int64_t)kSms * 4 / std::max<int64_t>(1, cols * groups);
-    p->team_items = 0;
     p->split = (int)std::max<int64_t>(1, std::min<int64_t>(want, p->group));
   } else {
-    const Tier t = tier_of(p->width, backward);
+    const Pass pass = backward ? BWD : FWD;
+    const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec));
+    teams = t.teams();
     // A team's items where a group has too few rows to keep a block's teams busy and there
-    // are groups enough to fill the GPU without splitting them.
-    p->team_items = p->group < 2 * t.teams() && groups >= 2 * kSms;
-    const int64_t want = full_grid(t, backward) / groups;  // one wave of blocks
-    const int64_t most = (p->group + t.teams() - 1) / t.teams();
+    // are groups enough for every SM.
+    p->team_items = p->group < 2 * teams && groups >= kSms * teams;
+    const int64_t want = (int64_t)kSms * bound_blocks(t.tpr, t.n, pass) / groups;  // one wave of blocks
+    const int64_t most = (p->group + teams - 1) / teams;
     p->split = p->team_items ? 1 : (int)std::max<int64_t>(1, std::min(want, most));
   }
   p->items = groups * p->split;
-  set_loop(p, p->group, p->team_items ? 1 : (int64_t)p->split * (is_wide(*p, x_type) ? 1 : tier_of(p->width, backward).teams()));
+  set_loop(p, p->group, p->team_items ? 1 : p->split * teams);
 }
 
 size_t workspace_bytes(const NormArgs& p) {
   return p.split > 1 ? (size_t)p.items * 2 * (size_t)p.width * sizeof(float) : 0;
 }
 
-cudaError_t launch_norm(NormArgs p, int x_type, bool backward, cudaStream_t st) {
+// Whether rows move as 16-byte vectors; sets p_vec.
+bool vector_rows(NormArgs* q, int x_type, bool backward) {
+  NormArgs& p = *q;
   const int64_t size = type_size(x_type), vec_elems = 16 / size;
   auto aligned = [](const void* q, int64_t stride_bytes, int64_t to) {
     return !q || ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)stride_bytes) & (uintptr_t)(to - 1)) == 0;
@@ -110,6 +115,10 @@ cudaError_t launch_norm(NormArgs p, int x_type, bool backward, cudaStream_t st) 
   p.p_vec = aligned(p.a, p.a_stride * ps, to) && aligned(p.b, p.b_stride * ps, to) &&
             aligned(p.da, p.width * ps, to) && aligned(p.db, p.width * ps, to) && (p.width * ps) % to == 0;
   if (p.one_plus && p.group == 1) vec = vec && p.p_vec;  // the ring moves both the same way
+  return vec;
+}
+
+cudaError_t launch_norm(const NormArgs& p, int x_type, bool backward, bool vec, cudaStream_t st) {
   const bool wide = is_wide(p, x_type);
   cudaError_t e = x_type == LEWM_TYPE_F32    ? launch_norm_rows<float>(p, wide, backward, vec, st)
                   : x_type == LEWM_TYPE_BF16 ? launch_norm_rows<__nv_bfloat16>(p, wide, backward, vec, st)
@@ -195,8 +204,10 @@ using namespace lewm;
 extern "C" size_t lewm_norm_workspace(const lewm_norm_desc* desc) {
   NormArgs p;
   if (norm_args(desc, &p) != LEWM_OK || p.rows == 0) return 0;
-  cut_items(&p, desc->x_type, true);
-  return workspace_bytes(p);
+  cut_items(&p, desc->x_type, true, true);
+  const size_t vec = workspace_bytes(p);
+  cut_items(&p, desc->x_type, true, false);
+  return std::max(vec, workspace_bytes(p));  // whichever way the tensors lie
 }
 
 extern "C" lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void* x, const void* a, const void* b,
@@ -217,8 +228,9 @@ extern "C" lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void*
   p.b = b;
   p.out = y;
   p.stats = stats;
-  cut_items(&p, desc->x_type, false);
-  const cudaError_t e = launch_norm(p, desc->x_type, false, static_cast<cudaStream_t>(stream));
+  const bool vec = vector_rows(&p, desc->x_type, false);
+  cut_items(&p, desc->x_type, false, vec);
+  const cudaError_t e = launch_norm(p, desc->x_type, false, vec, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return norm_fail(LEWM_CUDA_ERROR, "norm forward launch: %s", cudaGetErrorString(e));
   return LEWM_OK;
 }
@@ -239,17 +251,9 @@ extern "C" lewm_status lewm_norm_backward(const lewm_norm_desc* desc, const void
   }
   if (!dy || !x || !stats) return norm_fail(LEWM_INVALID_ARG, "dy, x and stats must be non-NULL");
   if (p.one_plus && !a) return norm_fail(LEWM_INVALID_ARG, "scale must be non-NULL");
-  cut_items(&p, desc->x_type, true);
-  if ((da || db) && workspace_bytes_given < workspace_bytes(p))
-    return norm_fail(LEWM_INVALID_ARG, "workspace of %zu bytes, needs %zu", workspace_bytes_given, workspace_bytes(p));
-  if ((da || db) && p.split > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
-    return norm_fail(LEWM_INVALID_ARG, "workspace must be non-NULL and 16-byte aligned");
   if (!on_elements(desc->x_type, {dy, x, dx}) || !on_elements(desc->p_type, {a, da, db}) ||
       !on_elements(LEWM_TYPE_F32, {stats}))
     return norm_fail(LEWM_INVALID_ARG, "a pointer is not aligned to its element type");
-  NormDevice nd(device);
-  if (nd.err != cudaSuccess)
-    return norm_fail(LEWM_CUDA_ERROR, "cudaSetDevice(%d): %s", device, cudaGetErrorString(nd.err));
   p.x = x;
   p.dy = dy;
   p.dy_stride = dy_stride;
@@ -259,7 +263,16 @@ extern "C" lewm_status lewm_norm_backward(const lewm_norm_desc* desc, const void
   p.db = db;
   p.stats = const_cast<float*>(stats);
   p.ws = static_cast<float*>(workspace);
-  const cudaError_t e = launch_norm(p, desc->x_type, true, static_cast<cudaStream_t>(stream));
+  const bool vec = vector_rows(&p, desc->x_type, true);
+  cut_items(&p, desc->x_type, true, vec);
+  if ((da || db) && workspace_bytes_given < workspace_bytes(p))
+    return norm_fail(LEWM_INVALID_ARG, "workspace of %zu bytes, needs %zu", workspace_bytes_given, workspace_bytes(p));
+  if ((da || db) && p.split > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return norm_fail(LEWM_INVALID_ARG, "workspace must be non-NULL and 16-byte aligned");
+  NormDevice nd(device);
+  if (nd.err != cudaSuccess)
+    return norm_fail(LEWM_CUDA_ERROR, "cudaSetDevice(%d): %s", device, cudaGetErrorString(nd.err));
+  const cudaError_t e = launch_norm(p, desc->x_type, true, vec, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return norm_fail(LEWM_CUDA_ERROR, "norm backward launch: %s", cudaGetErrorString(e));
   return LEWM_OK;
 }

@@ -46,6 +46,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "lewm_b200.h"
@@ -107,16 +108,61 @@ __device__ __forceinline__ void store_param(void* p, int type, int64_t at, float
 // ------------------------------------------------------------------ teams
 constexpr int block_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 
-// What a thread holds of a row. N values as N / 2 pairs: vector i of the team's vectors lane +
-// i TPR, whose E values are pairs i E / 2 on (E > 1); or single values lane + i TPR, two of
-// consecutive i in a pair (E = 1).
-template <int E_, int NV_, int TPR_>
+// Passes: an item's rows share their parameters, or each row has its own modulation row.
+enum Pass { FWD, BWD, ROW_FWD, ROW_BWD };
+constexpr bool is_backward(Pass p) { return p == BWD || p == ROW_BWD; }
+
+// Team of a row: threads x values a thread cover the width.
+struct Tier {
+  int tpr, n;
+  constexpr int teams() const { return block_threads(tpr) / tpr; }
+};
+// Many narrow rows take small teams of many values (`dense`), so several rows to a warp: a row costs a
+// thread some hundred instructions beside those of its values, and a team of 32 spends them 32
+// times (57600 x 192 bf16 with a modulation row per row: forward 19.0 us in teams of 32, 15.9 in teams
+// of 8; 16448 x 192 forward 6.9 and 5.8). Fewer rows than fill the GPU that way keep teams of 32, whose
+// threads have less to do one after the other (900 x 192 float32 forward 3.1 us, 4.8 in teams of 8), and
+// so do rows at odd addresses, whose single-element accesses are then 64 bytes wide.
+constexpr bool dense_rows(int64_t rows, bool vec) { return vec && rows >= 32 * kSms; }
+constexpr Tier tier_of(int64_t width, Pass pass, bool dense) {
+  if (width <= 64) return {8, 8};
+  if (!dense) {
+    if (width <= 256) return {32, 8};
+  } else {
+    if (width <= 128) return {8, 16};
+    if (width <= 192 && pass != BWD) return {8, 24};
+    if (width <= 256) return {16, 16};
+    if (width <= 384 && pass != BWD) return {16, 24};
+  }
+  // The forward keeps no sums: 32 values a thread leave two blocks per SM where 16 leave one.
+  if (!is_backward(pass) && width > 4096 && width <= 8192) return {256, 32};
+  int tpr = 32;
+  while (tpr * 16 < width) tpr *= 2;  // rows of at most kMaxRowBytes: tpr <= 1024
+  return {tpr, 16};
+}
+// The narrowest row of a tier, 0 for one that the pass does not use. (The tiers that dense rows and
+// others share have the same narrowest row, or the lower one.)
+constexpr int64_t min_width_of(int tpr, int n, Pass pass, bool dense) {
+  const int64_t edges[] = {64, 128, 192, 256, 384, 512, 1024, 2048, 4096, 8192, 16384};
+  int64_t before = 0;
+  for (int64_t e : edges) {
+    const Tier t = tier_of(e, pass, dense);
+    if (t.tpr == tpr && t.n == n) return before + 1;
+    before = e;
+  }
+  return 0;
+}
+constexpr int64_t min_width(int tpr, int n, Pass pass, bool vec) {
+  const int64_t a = min_width_of(tpr, n, pass, false), b = vec ? min_width_of(tpr, n, pass, true) : 0;
+  return a == 0 ? b : b == 0 || a < b ? a : b;
+}
+
+template <int E_, int NV_, int TPR_, int64_t MIN_WIDTH>
 struct Team {
   static constexpr int E = E_, NV = NV_, TPR = TPR_, N = E * NV, H = N / 2;
   static constexpr int THREADS = block_threads(TPR), TEAMS = THREADS / TPR;
-  // Vectors that lie inside every row of the tier: its narrowest row fills more than half of a
-  // team (a quarter in the tier of 65 to 256).
-  static constexpr int SURE = TPR == 8 ? 0 : N == 8 ? NV / 4 : NV / 2;
+  // Vectors that lie inside every row of the tier.
+  static constexpr int SURE = (int)(MIN_WIDTH / (TPR * E));
 
   static __device__ __forceinline__ int team() { return threadIdx.x / TPR; }
   static __device__ __forceinline__ int lane() { return threadIdx.x % TPR; }
@@ -392,17 +438,16 @@ struct Walk {
         step(step_rows * stride) {}
 };
 
-// Blocks per SM that the registers are limited for: 80 a thread forward (128 with 32 values), 128 in
-// the backward that keeps sums. More, smaller blocks were slower on short rows (16448 x 192 bf16 forward, 3, 4 and 5
-// blocks: 6.8, 6.9, 7.2 us): every block loads the parameters anew. The backward of a modulation
-// row per row has neither and takes 4 there (57600 x 192 bf16, 2, 3 and 4 blocks: 26.2, 22.9,
-// 21.6 us).
-template <typename Tm>
-constexpr int bound_blocks(bool backward, bool rowmod = false) {
-  if (rowmod && backward && Tm::N == 8) return 4;
-  const int n = (backward || Tm::N == 32 ? 512 : 768) / Tm::THREADS;
-  return n > 0 ? n : 1;
+// Blocks per SM that the registers are limited for: 80 a thread forward (128 with 24 or 32 values), 128
+// in the backward that keeps sums. More, smaller blocks were slower on short rows: every block
+// loads the parameters anew. The backward of a modulation row per row has neither and takes 4
+// with 8 values (57600 x 192 bf16 in teams of 32, 2, 3 and 4 blocks: 26.2, 22.9, 21.6 us).
+constexpr int bound_blocks(int tpr, int n, Pass pass) {
+  const int threads = pass == ROW_BWD && n == 8 ? 1024 : is_backward(pass) || n >= 24 ? 512 : 768;
+  return threads >= block_threads(tpr) ? threads / block_threads(tpr) : 1;
 }
+template <typename Tm, Pass PASS>
+constexpr int kBound = bound_blocks(Tm::TPR, Tm::N, PASS);
 
 // What multiplies z in group g, and what is added: weight or 1 + scale, bias or shift.
 template <typename Tm>
@@ -423,6 +468,15 @@ __device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b)
 }
 
 // ------------------------------------------------------------------ forward
+// 1 / sqrt(t): the GPU's approximation (2 ulp) and a Newton step for t^-1/2, r (3 - t r^2) / 2, which
+// leaves about one rounding; a third of the instructions of a division and a root. 0 and infinity
+// stay as they are.
+__device__ __forceinline__ float inv_sqrt(float t) {
+  const float r = rsqrtf(t);
+  const float n = r * fmaf(-0.5f * t, r * r, 1.5f);
+  return t > 0.f && t < INFINITY ? n : r;
+}
+
 // x - mu in place of the team's values x (0 beyond the row), mu and rs.
 template <typename Tm>
 __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float (*red)[32]) {
@@ -450,11 +504,11 @@ __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float
     }
   }
   const float var = Tm::sum(both(q), red[1]) * inv_n;
-  return make_float2(mu, 1.0f / sqrtf(var + eps));
+  return make_float2(mu, inv_sqrt(var + eps));
 }
 
 template <typename T, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_norm_fwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, FWD>) k_norm_fwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
   using St = Stage<T, Tm>;
   constexpr int H = Tm::H;
@@ -518,7 +572,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_norm_f
 
 // A modulation row per row of x: rows in a grid stride, scale and shift in the ring beside x.
 template <typename T, typename P, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(false)) k_rowmod_fwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_FWD>) k_rowmod_fwd(const NormArgs p) {
   griddep_wait();
   using St = Stage<T, Tm>;
   using Sp = Stage<P, Tm>;
@@ -594,7 +648,7 @@ __device__ __forceinline__ void store_dx(T* dx, int width, const F2* z, F2* d, f
 }
 
 template <typename T, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true)) k_norm_bwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, BWD>) k_norm_bwd(const NormArgs p) {
   griddep_wait();  // launched as a programmatic dependent: wait for the kernel before
   // The whole grid is resident by now, so the reduction's blocks take no slot from it; they
   // wait for its end with their launch behind them.
@@ -728,7 +782,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true)) k_norm_bw
 
 // A modulation row per row of x: d scale = dy z and d shift = dy row by row, nothing to sum up.
 template <typename T, typename P, typename Tm>
-__global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true, true)) k_rowmod_bwd(const NormArgs p) {
+__global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_BWD>) k_rowmod_bwd(const NormArgs p) {
   griddep_wait();
   using St = Stage<T, Tm>;
   using Sp = Stage<P, Tm>;
@@ -810,7 +864,7 @@ __global__ void __launch_bounds__(Tm::THREADS, bound_blocks<Tm>(true, true)) k_r
 
 // ------------------------------------------------------------------ rows of more than kMaxRowBytes
 // A block per row, the row re-read (from L2) for each pass, in vectors of E elements.
-using Wide = Team<1, 2, 1024>;
+using Wide = Team<1, 2, 1024, 0>;
 
 // E elements of T at `q` as float32.
 template <typename T, int E>
@@ -867,7 +921,7 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) q = fmaf(f[e] - mu, f[e] - mu, q);
     }
-    const float rs = 1.0f / sqrtf(Wide::sum(q, red[1]) * inv_n + p.eps);
+    const float rs = inv_sqrt(Wide::sum(q, red[1]) * inv_n + p.eps);
     if (p.stats && threadIdx.x == 0) {
       p.stats[r] = mu;
       p.stats[p.rows + r] = rs;
@@ -973,30 +1027,9 @@ __global__ void __launch_bounds__(256) k_norm_sums_wide(const NormArgs p) {
 }
 
 // ------------------------------------------------------------------ host side
-// Team of a row: threads x elements per thread covers the width.
-struct Tier {
-  int tpr, ept;
-  int teams() const { return block_threads(tpr) / tpr; }
-};
-inline Tier tier_of(int64_t width, bool backward) {
-  if (width <= 64) return {8, 8};
-  if (width <= 256) return {32, 8};
-  // The forward keeps no sums: 32 values a thread leave two blocks per SM where 16 leave one.
-  if (!backward && width > 4096 && width <= 8192) return {256, 32};
-  int tpr = 32;
-  while (tpr * 16 < width) tpr *= 2;  // rows of at most kMaxRowBytes: tpr <= 1024
-  return {tpr, 16};
-}
 inline int64_t type_size(int type) { return type == LEWM_TYPE_F32 ? 4 : 2; }
 inline bool is_wide(const NormArgs& p, int x_type) { return p.width * type_size(x_type) > kMaxRowBytes; }
 
-// Blocks that fill the GPU once.
-inline int64_t full_grid(const Tier& t, bool backward) {
-  return (int64_t)kSms * (t.ept == 32      ? bound_blocks<Team<1, 32, 256>>(backward)
-                          : t.tpr <= 256   ? bound_blocks<Team<1, 16, 256>>(backward)
-                          : t.tpr == 512   ? bound_blocks<Team<1, 16, 512>>(backward)
-                                           : bound_blocks<Team<1, 16, 1024>>(backward));
-}
 // Rounds of loops over `rows` rows in steps of `step`. (No tensor that fits a GPU makes 2^31 rounds: a
 // step is a row for groups of a few, else a block's teams times the blocks that share the rows.)
 inline void set_loop(NormArgs* p, int64_t rows, int64_t step) {
@@ -1036,72 +1069,75 @@ cudaError_t launch_ring(K kern, std::atomic<bool>* raised, int64_t grid, int thr
   return launch_k(kern, dim3((unsigned)grid), dim3(threads), smem, st, p);
 }
 
-// The passes that use a tier (tier_of).
-template <typename Tm>
-constexpr bool has_backward = Tm::N != 32;
-template <typename Tm>
-constexpr bool has_forward = !(Tm::N == 16 && Tm::TPR == 512);
-
-template <typename T, typename Tm>
-cudaError_t launch_items(NormArgs p, bool backward, cudaStream_t st) {
-  static std::atomic<bool> raised[2][64];
-  const int bytes = (backward ? 2 : 1) * Stage<T, Tm>::BYTES;
-  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward), backward ? kAheadBackward : kAhead);
-  const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
-  const int64_t grid = std::min(blocks, (int64_t)kSms * bound_blocks<Tm>(backward));
-  if constexpr (has_backward<Tm>)
-    if (backward) return launch_ring(k_norm_bwd<T, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st);
-  if constexpr (has_forward<Tm>)
-    if (!backward) return launch_ring(k_norm_fwd<T, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
-  return cudaErrorInvalidValue;  // not a tier of this pass
+// One pass of a tier, if the pass uses it: sets *e and returns true.
+template <typename T, typename P, int E, Pass PASS, int TPR, int N>
+bool launch_tier(const Tier& t, NormArgs p, cudaStream_t st, cudaError_t* e) {
+  constexpr int64_t MIN = min_width(TPR, N, PASS, E > 1);
+  if constexpr (MIN > 0 && N % E == 0 && MIN * (int)sizeof(T) <= kMaxRowBytes) {
+    if (t.tpr != TPR || t.n != N) return false;
+    using Tm = Team<E, N / E, TPR, MIN>;
+    static std::atomic<bool> raised[64];
+    constexpr int x_bytes = Stage<T, Tm>::BYTES, p_bytes = Stage<P, Tm>::BYTES;
+    constexpr int bytes = PASS == FWD       ? x_bytes
+                          : PASS == BWD     ? 2 * x_bytes
+                          : PASS == ROW_FWD ? x_bytes + 2 * p_bytes
+                                            : 2 * x_bytes + p_bytes;
+    p.stages = ring_stages(bytes, kBound<Tm, PASS>, PASS == BWD ? kAheadBackward : kAhead);
+    if (p.stages == 0) return false;  // modulation too wide for the ring
+    const int64_t full = (int64_t)kSms * kBound<Tm, PASS>;
+    if constexpr (PASS == FWD || PASS == BWD) {
+      const int64_t blocks = p.team_items ? (p.items + Tm::TEAMS - 1) / Tm::TEAMS : p.items;
+      const int64_t grid = std::min(blocks, full);
+      if constexpr (PASS == FWD) *e = launch_ring(k_norm_fwd<T, Tm>, raised, grid, Tm::THREADS, bytes * p.stages, p, st);
+      else *e = launch_ring(k_norm_bwd<T, Tm>, raised, grid, Tm::THREADS, bytes * p.stages, p, st);
+    } else {
+      const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, full);
+      set_loop(&p, p.rows, grid * Tm::TEAMS);
+      if constexpr (PASS == ROW_FWD)
+        *e = launch_ring(k_rowmod_fwd<T, P, Tm>, raised, grid, Tm::THREADS, bytes * p.stages, p, st);
+      else *e = launch_ring(k_rowmod_bwd<T, P, Tm>, raised, grid, Tm::THREADS, bytes * p.stages, p, st);
+    }
+    return true;
+  }
+  return false;
 }
 
-// group 1: the modulation in the ring, if two stages of it fit.
-template <typename T, typename P, typename Tm>
-cudaError_t launch_rowmod(NormArgs p, bool backward, cudaStream_t st) {
-  static std::atomic<bool> raised[2][64];
-  const int x_bytes = Stage<T, Tm>::BYTES, p_bytes = Stage<P, Tm>::BYTES;
-  const int bytes = backward ? 2 * x_bytes + p_bytes : x_bytes + 2 * p_bytes;
-  p.stages = ring_stages(bytes, bound_blocks<Tm>(backward, true), kAhead);
-  if (p.stages == 0) return launch_items<T, Tm>(p, backward, st);
-  const int64_t grid = std::min((p.rows + Tm::TEAMS - 1) / Tm::TEAMS, (int64_t)kSms * bound_blocks<Tm>(backward, true));
-  set_loop(&p, p.rows, grid * Tm::TEAMS);
-  if constexpr (has_backward<Tm>)
-    if (backward) return launch_ring(k_rowmod_bwd<T, P, Tm>, raised[1], grid, Tm::THREADS, bytes * p.stages, p, st);
-  if constexpr (has_forward<Tm>)
-    if (!backward) return launch_ring(k_rowmod_fwd<T, P, Tm>, raised[0], grid, Tm::THREADS, bytes * p.stages, p, st);
-  return cudaErrorInvalidValue;  // not a tier of this pass
+template <typename T, typename P, int E, Pass PASS>
+bool launch_pass(const NormArgs& p, cudaStream_t st, cudaError_t* e) {
+  const Tier t = tier_of(p.width, PASS, dense_rows(p.rows, E > 1));
+  return launch_tier<T, P, E, PASS, 8, 8>(t, p, st, e) || launch_tier<T, P, E, PASS, 8, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 8, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 16, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 16, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 8>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 32, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 128, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 256, 32>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 1024, 16>(t, p, st, e);
 }
-
-template <typename T, int E, int NV, int TPR>
-cudaError_t launch_tier(const NormArgs& p, bool backward, cudaStream_t st) {
-  using Tm = Team<E, NV, TPR>;
-  if (p.group > 1 || !p.one_plus) return launch_items<T, Tm>(p, backward, st);
-  if (p.p_type == LEWM_TYPE_F32) return launch_rowmod<T, float, Tm>(p, backward, st);
-  constexpr bool any = std::is_same<T, float>::value;
-  if constexpr (any || std::is_same<T, __nv_bfloat16>::value)
-    if (p.p_type == LEWM_TYPE_BF16) return launch_rowmod<T, __nv_bfloat16, Tm>(p, backward, st);
-  if constexpr (any || std::is_same<T, __half>::value)
-    if (p.p_type == LEWM_TYPE_F16) return launch_rowmod<T, __half, Tm>(p, backward, st);
-  return launch_items<T, Tm>(p, backward, st);  // bf16 beside fp16
+template <typename T, typename P, int E>
+bool launch_rows_mod(const NormArgs& p, bool backward, cudaStream_t st, cudaError_t* e) {
+  return backward ? launch_pass<T, P, E, ROW_BWD>(p, st, e) : launch_pass<T, P, E, ROW_FWD>(p, st, e);
 }
 
 template <typename T, int E>
 cudaError_t launch_width(const NormArgs& p, bool backward, cudaStream_t st) {
-  constexpr int V8 = 8 / E, V16 = 16 / E, V32 = 32 / E;
-  const Tier t = tier_of(p.width, backward);
-  if (t.ept == 8) return t.tpr == 8 ? launch_tier<T, E, V8, 8>(p, backward, st) : launch_tier<T, E, V8, 32>(p, backward, st);
-  if (t.ept == 32) return launch_tier<T, E, V32, 256>(p, false, st);
-  switch (t.tpr) {
-    case 32: return launch_tier<T, E, V16, 32>(p, backward, st);
-    case 64: return launch_tier<T, E, V16, 64>(p, backward, st);
-    case 128: return launch_tier<T, E, V16, 128>(p, backward, st);
-    case 256: return launch_tier<T, E, V16, 256>(p, backward, st);
-    case 512: return launch_tier<T, E, V16, 512>(p, backward, st);
-    default:
-      if constexpr (sizeof(T) == 2) return launch_tier<T, E, V16, 1024>(p, backward, st);
-      return cudaErrorInvalidValue;  // float32 rows this wide are more than kMaxRowBytes
+  cudaError_t e = cudaErrorInvalidValue;
+  // A modulation row per row of x: the modulation in the ring, if two stages of it fit. bf16 beside
+  // fp16 goes without.
+  if (p.one_plus && p.group == 1) {
+    constexpr bool any = std::is_same<T, float>::value;
+    if (p.p_type == LEWM_TYPE_F32) {
+      if (launch_rows_mod<T, float, E>(p, backward, st, &e)) return e;
+    }
+    if constexpr (any || std::is_same<T, __nv_bfloat16>::value) {
+      if (p.p_type == LEWM_TYPE_BF16 && launch_rows_mod<T, __nv_bfloat16, E>(p, backward, st, &e)) return e;
+    }
+    if constexpr (any || std::is_same<T, __half>::value) {
+      if (p.p_type == LEWM_TYPE_F16 && launch_rows_mod<T, __half, E>(p, backward, st, &e)) return e;
+    }
   }
+  if (backward) launch_pass<T, T, E, BWD>(p, st, &e);
+  else launch_pass<T, T, E, FWD>(p, st, &e);
+  return e;
 }
 
 template <typename T, int E>
