@@ -46,7 +46,6 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cmath>
 #include <type_traits>
 
 #include "lewm_b200.h"
@@ -468,15 +467,6 @@ __device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b)
 }
 
 // ------------------------------------------------------------------ forward
-// 1 / sqrt(t): the GPU's approximation (2 ulp) and a Newton step for t^-1/2, r (3 - t r^2) / 2, which
-// leaves about one rounding; a third of the instructions of a division and a root. 0 and infinity
-// stay as they are.
-__device__ __forceinline__ float inv_sqrt(float t) {
-  const float r = rsqrtf(t);
-  const float n = r * fmaf(-0.5f * t, r * r, 1.5f);
-  return t > 0.f && t < INFINITY ? n : r;
-}
-
 // x - mu in place of the team's values x (0 beyond the row), mu and rs.
 template <typename Tm>
 __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float (*red)[32]) {
@@ -504,7 +494,7 @@ __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float
     }
   }
   const float var = Tm::sum(both(q), red[1]) * inv_n;
-  return make_float2(mu, inv_sqrt(var + eps));
+  return make_float2(mu, 1.0f / sqrtf(var + eps));
 }
 
 template <typename T, typename Tm>
@@ -921,7 +911,7 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) q = fmaf(f[e] - mu, f[e] - mu, q);
     }
-    const float rs = inv_sqrt(Wide::sum(q, red[1]) * inv_n + p.eps);
+    const float rs = 1.0f / sqrtf(Wide::sum(q, red[1]) * inv_n + p.eps);
     if (p.stats && threadIdx.x == 0) {
       p.stats[r] = mu;
       p.stats[p.rows + r] = rs;
