@@ -58,24 +58,8 @@ namespace lewm {
 namespace {
 
 // ------------------------------------------------------------------ parameters
-// E elements of type P at `q` as pairs (E > 1), in accesses of min(16, E sizeof(P)) bytes if the
+// E values as elements of type P at `q` (E > 1), in accesses of min(16, E sizeof(P)) bytes if the
 // address allows it (`vec`).
-template <typename P, int E>
-__device__ __forceinline__ void load_pairs(const P* q, bool vec, F2* f) {
-  constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
-#pragma unroll
-  for (int k = 0; k < E / N; ++k) {
-    Vec<P, N> v;
-    if (vec) {
-      v = reinterpret_cast<const Vec<P, N>*>(q)[k];
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) v.v[e] = q[k * N + e];
-    }
-#pragma unroll
-    for (int e = 0; e < N; e += 2) f[(k * N + e) / 2] = unpack(v.v + e);
-  }
-}
 template <typename P, int E>
 __device__ __forceinline__ void store_pairs(P* q, bool vec, const F2* f) {
   constexpr int N = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E;
@@ -208,30 +192,47 @@ struct Team {
     return v;
   }
 
-  // This thread's parameters of a row of `width` at element offset `at`, `outside` beyond it.
-  static __device__ __forceinline__ void load_params(const void* p, int type, int64_t at, int width, bool vec, F2* f) {
+  // This thread's parameters of a row of `width`, 0 beyond it. All loads before the first conversion:
+  // one after the other they cost a block several us.
+  template <typename P>
+  static __device__ __forceinline__ void load_typed(const P* q, int width, bool vec, F2* f) {
     if constexpr (E > 1) {
+      constexpr int K = E * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : E, PIECES = E / K;
       const int nvec = width / E;
+      Vec<P, K> raw[NV][PIECES] = {};
+      q += lane() * E;
+      if (vec) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = lane() + i * TPR;
-        if (v >= nvec) continue;
-        F2* o = f + i * (E / 2);
-        const int64_t c = at + (int64_t)v * E;
-        if (type == LEWM_TYPE_F32) load_pairs<float, E>(static_cast<const float*>(p) + c, vec, o);
-        else if (type == LEWM_TYPE_BF16) load_pairs<__nv_bfloat16, E>(static_cast<const __nv_bfloat16*>(p) + c, vec, o);
-        else load_pairs<__half, E>(static_cast<const __half*>(p) + c, vec, o);
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k)
+            if (i < SURE || lane() + i * TPR < nvec) raw[i][k] = reinterpret_cast<const Vec<P, K>*>(q + i * TPR * E)[k];
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (i < SURE || lane() + i * TPR < nvec) raw[i][e / K].v[e % K] = q[i * TPR * E + e];
       }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+#pragma unroll
+          for (int e = 0; e < K; e += 2) f[(i * E + k * K + e) / 2] = unpack(raw[i][k].v + e);
     } else {
+      P raw[N] = {};
 #pragma unroll
-      for (int i = 0; i < H; ++i) {
-        const int c = lane() + 2 * i * TPR;
-        float2 v = split(f[i]);
-        if (c < width) v.x = load_param(p, type, at + c);
-        if (c + TPR < width) v.y = load_param(p, type, at + c + TPR);
-        f[i] = f2(v.x, v.y);
-      }
+      for (int i = 0; i < N; ++i)
+        if (i < SURE || lane() + i * TPR < width) raw[i] = q[lane() + i * TPR];
+#pragma unroll
+      for (int i = 0; i < H; ++i) f[i] = f2(to_f(raw[2 * i]), to_f(raw[2 * i + 1]));
     }
+  }
+  static __device__ __forceinline__ void load_params(const void* p, int type, int64_t at, int width, bool vec, F2* f) {
+    if (type == LEWM_TYPE_F32) load_typed(static_cast<const float*>(p) + at, width, vec, f);
+    else if (type == LEWM_TYPE_BF16) load_typed(static_cast<const __nv_bfloat16*>(p) + at, width, vec, f);
+    else load_typed(static_cast<const __half*>(p) + at, width, vec, f);
   }
   // Stores a row of `width` values of type P at `row`.
   template <typename P>
@@ -451,9 +452,12 @@ constexpr int kBound = bound_blocks(Tm::TPR, Tm::N, PASS);
 // What multiplies z in group g, and what is added: weight or 1 + scale, bias or shift.
 template <typename Tm>
 __device__ __forceinline__ void load_gain(const NormArgs& p, int64_t g, F2* a) {
+  if (p.a) {
+    Tm::load_params(p.a, p.p_type, g * p.a_stride, p.width, p.p_vec, a);
+  } else {
 #pragma unroll
-  for (int k = 0; k < Tm::H; ++k) a[k] = f2(p.one_plus ? 0.f : 1.f);
-  if (p.a) Tm::load_params(p.a, p.p_type, g * p.a_stride, p.width, p.p_vec, a);
+    for (int k = 0; k < Tm::H; ++k) a[k] = f2(1.f);
+  }
   if (p.one_plus) {
 #pragma unroll
     for (int k = 0; k < Tm::H; ++k) a[k] = a[k] + f2(1.f);
@@ -461,9 +465,12 @@ __device__ __forceinline__ void load_gain(const NormArgs& p, int64_t g, F2* a) {
 }
 template <typename Tm>
 __device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b) {
+  if (p.b) {
+    Tm::load_params(p.b, p.p_type, g * p.b_stride, p.width, p.p_vec, b);
+  } else {
 #pragma unroll
-  for (int k = 0; k < Tm::H; ++k) b[k] = f2(0.f);
-  if (p.b) Tm::load_params(p.b, p.p_type, g * p.b_stride, p.width, p.p_vec, b);
+    for (int k = 0; k < Tm::H; ++k) b[k] = f2(0.f);
+  }
 }
 
 // ------------------------------------------------------------------ forward
