@@ -10,15 +10,17 @@
 // (a, b) per `group` consecutive rows. Both are the same computation over groups of rows that
 // share (a, b), with one group for layer norm, so one kernel each way serves both.
 //
-// Bound: bytes. About 10 (forward) and 16 (backward) instructions per element against 4 to 12
-// bytes of HBM traffic. A row therefore stays in registers from its only load to its only
+// Bound: bytes, 4 to 12 per element and pass. Many rows run at 91 to 102% of the rate of a plain copy
+// (131072 x 2048 bf16: forward 172 us, backward 261; 73881 x 1536 float32, groups of 8209 rows: 140 and
+// 203), at odd addresses at about 60%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
+// 35 and 52 us). A row therefore stays in registers from its only load to its only
 // store (mean and variance are two passes over registers), and sums over rows are kept in
 // registers by persistent blocks that own fixed columns, so x and dy are read once.
 //
 // Layout: a team of TPR threads holds one row, NV vectors of E elements per thread (16-byte
-// vectors where every row starts on 16 bytes, else single elements), at most 16 elements a
-// thread: the backward then holds 16 gains and 32 sums, 128 registers at two 256-thread blocks
-// per SM. Rows of more than 32 KB take the looping kernels below.
+// vectors where every row starts on 16 bytes, else single elements). In the backward that is at
+// most 16 elements a thread: it then holds 16 gains and 32 sums, 128 registers at two 256-thread
+// blocks per SM. Rows of more than 32 KB take the looping kernels below.
 //
 // Rows arrive through a ring of 2 to 4 stages in shared memory, filled by cp.async one to
 // three rows ahead: registers alone kept 32 KB per SM on the way at best and none while a row
