@@ -37,13 +37,14 @@ __global__ void __launch_bounds__(256) k_norm_reduce(const NormArgs p) {
     for (int e = 0; e < VW; ++e) s.v[e] = 0.f;
     if (col < p.width) {
       const float* w = p.ws + (g * p.split * 2 + blockIdx.z) * p.width + col;
-      for (int i = run; i < p.split; i += 8 * R) {
-        V v[8];
+      constexpr int B = 12;  // loads in flight
+      for (int i = run; i < p.split; i += B * R) {
+        V v[B];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < B; ++k)
           if (i + k * R < p.split) v[k] = *reinterpret_cast<const V*>(w + (i + k * R) * stride);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < B; ++k)
           if (i + k * R < p.split) {
 #pragma unroll
             for (int e = 0; e < VW; ++e) s.v[e] += v[k].v[e];
