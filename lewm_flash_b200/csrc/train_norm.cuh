@@ -476,14 +476,16 @@ __device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b)
 }
 
 // ------------------------------------------------------------------ forward
-// x - mu in place of the team's values x (0 beyond the row), mu and rs.
+// x - mu in place of the team's values x (0 beyond the row), mu and rs. The mean is divided, not
+// multiplied by 1 / n: that of a constant row (padding) is then the constant, and z is 0, where one
+// rounding of mu would come out as rs = 1 / sqrt(eps) times itself.
 template <typename Tm>
 __device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float (*red)[32]) {
   constexpr int E = Tm::E, TPR = Tm::TPR;
   F2 s = f2(0.f), q = f2(0.f);
 #pragma unroll
   for (int k = 0; k < Tm::H; ++k) s = s + f[k];
-  const float mu = Tm::sum(both(s), red[0]) * inv_n;
+  const float mu = Tm::sum(both(s), red[0]) / (float)width;
   const F2 nm = f2(-mu);
 #pragma unroll
   for (int k = 0; k < Tm::H; ++k) {
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) s += f[e];
     }
-    const float mu = Wide::sum(s, red[0]) * inv_n;
+    const float mu = Wide::sum(s, red[0]) / (float)p.width;
 #pragma unroll 4
     for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
       load_f<T, E>(x + c, f);

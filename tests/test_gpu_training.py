@@ -223,6 +223,15 @@ def test_large_offset_keeps_the_variance():
     check_norm(x, None, None, 1e-5, False, 0, y.detach(), dy, dx, None, None)
 
 
+@pytest.mark.parametrize("width", [1, 3, 192, 1011, 1536, 20000])
+def test_constant_rows_give_the_bias(width):
+    """Whole numbers whose sums are exact: mean and variance are too, so z is 0 and y the bias."""
+    x = torch.tensor([0.0, 1.0, -7.0, 100.0], device=DEV)[:, None].expand(4, width).contiguous()
+    w, b = randn(width, seed=1), randn(width, seed=2)
+    assert torch.equal(lf.layer_norm(x, w, b), b.expand(4, -1))
+    assert torch.equal(lf.ada_layer_norm(x, b, w), b.expand(4, -1))
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the 64-bit forward, central differences: step h leaves h^2 / 6 of a
     third derivative of order 10, so 1e-6 at h = 1e-4 is far under the float32 gradients' 1e-5."""
