@@ -10,9 +10,9 @@
 
 namespace lewm {
 
-extern template cudaError_t launch_norm_rows<float>(const NormArgs&, bool, bool, bool, cudaStream_t);
-extern template cudaError_t launch_norm_rows<__nv_bfloat16>(const NormArgs&, bool, bool, bool, cudaStream_t);
-extern template cudaError_t launch_norm_rows<__half>(const NormArgs&, bool, bool, bool, cudaStream_t);
+extern template cudaError_t launch_norm_rows<float>(const NormArgs&, bool, bool, int, cudaStream_t);
+extern template cudaError_t launch_norm_rows<__nv_bfloat16>(const NormArgs&, bool, bool, int, cudaStream_t);
+extern template cudaError_t launch_norm_rows<__half>(const NormArgs&, bool, bool, int, cudaStream_t);
 
 namespace {
 
@@ -73,8 +73,31 @@ __global__ void __launch_bounds__(256) k_norm_reduce(const NormArgs p) {
   }
 }
 
+// Items per group: the fewest that come within 5% of the least rounds of rows that one of `full`
+// resident blocks goes through, where an item costs about four rounds beside its rows (its loads from
+// cold) and a backward's second launch eight. 340 groups of 139 rows on 296 blocks run in 2 waves of 139
+// rounds undivided, 3 of 70 in halves.
+int64_t best_split(int64_t groups, int64_t group, int64_t teams, int64_t full, bool backward) {
+  const int64_t most = (group + teams - 1) / teams;
+  auto cost = [&](int64_t split) {
+    const int64_t waves = (groups * split + full - 1) / full, rounds = (group + split * teams - 1) / (split * teams);
+    return waves * (rounds + 4) + (backward && split > 1 ? 8 : 0);
+  };
+  auto clamp = [&](int64_t split) { return std::max<int64_t>(1, std::min(split, most)); };
+  int64_t best = 1;
+  for (int64_t waves = 1; waves <= 8; ++waves) {
+    const int64_t split = clamp(waves * full / groups);
+    if (cost(split) < cost(best)) best = split;
+  }
+  for (int64_t waves = 1; waves <= 8; ++waves) {
+    const int64_t split = clamp(waves * full / groups);
+    if (split < best && cost(split) * 100 <= cost(best) * 105) best = split;
+  }
+  return best;
+}
+
 // How rows are cut into items; the same function sizes the workspace.
-void cut_items(NormArgs* p, int x_type, bool backward, bool vec) {
+void cut_items(NormArgs* p, int x_type, bool backward, int vec) {
   const int64_t groups = p->rows / p->group;
   int64_t teams = 1;
   p->team_items = 0;
@@ -85,14 +108,12 @@ void cut_items(NormArgs* p, int x_type, bool backward, bool vec) {
     p->split = (int)std::max<int64_t>(1, std::min<int64_t>(want, p->group));
   } else {
     const Pass pass = backward ? BWD : FWD;
-    const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec));
+    const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec == 16));
     teams = t.teams();
     // A team's items where a group has too few rows to keep a block's teams busy and there
     // are groups enough for every SM.
     p->team_items = p->group < 2 * teams && groups >= kSms * teams;
-    const int64_t want = (int64_t)kSms * bound_blocks(t.tpr, t.n, pass) / groups;  // one wave of blocks
-    const int64_t most = (p->group + teams - 1) / teams;
-    p->split = p->team_items ? 1 : (int)std::max<int64_t>(1, std::min(want, most));
+    p->split = p->team_items ? 1 : (int)best_split(groups, p->group, teams, (int64_t)kSms * bound_blocks(t.tpr, t.n, pass), backward);
   }
   p->items = groups * p->split;
   set_loop(p, p->group, p->team_items ? 1 : p->split * teams);
@@ -102,24 +123,29 @@ size_t workspace_bytes(const NormArgs& p) {
   return p.split > 1 ? (size_t)p.items * 2 * (size_t)p.width * sizeof(float) : 0;
 }
 
-// Whether rows move as 16-byte vectors; sets p_vec.
-bool vector_rows(NormArgs* q, int x_type, bool backward) {
+// Bytes of the vectors that rows move in: 16, 8, 4 or an element's. Sets p_vec.
+int vector_bytes(NormArgs* q, int x_type, bool backward) {
   NormArgs& p = *q;
-  const int64_t size = type_size(x_type), vec_elems = 16 / size;
+  const int64_t size = type_size(x_type), ps = type_size(p.p_type);
   auto aligned = [](const void* q, int64_t stride_bytes, int64_t to) {
     return !q || ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)stride_bytes) & (uintptr_t)(to - 1)) == 0;
   };
-  bool vec = aligned(p.x, p.x_stride * size, 16) && aligned(p.out, p.width * size, 16) &&
-             (!backward || aligned(p.dy, p.dy_stride * size, 16)) && (p.width * size) % 16 == 0;
-  // A vector's parameters as 16-byte (8-byte: 16-bit ones beside float32 rows) accesses.
-  const int64_t ps = type_size(p.p_type), to = std::min<int64_t>(16, vec_elems * ps);
-  p.p_vec = aligned(p.a, p.a_stride * ps, to) && aligned(p.b, p.b_stride * ps, to) &&
-            aligned(p.da, p.width * ps, to) && aligned(p.db, p.width * ps, to) && (p.width * ps) % to == 0;
-  if (p.one_plus && p.group == 1) vec = vec && p.p_vec;  // the ring moves both the same way
-  return vec;
+  for (int vec = 16; vec > size; vec /= 2) {
+    if (!aligned(p.x, p.x_stride * size, vec) || !aligned(p.out, p.width * size, vec) || (p.width * size) % vec ||
+        (backward && !aligned(p.dy, p.dy_stride * size, vec)))
+      continue;
+    // A vector's parameters as accesses of up to 16 bytes.
+    const int64_t to = std::min<int64_t>(16, vec / size * ps);
+    p.p_vec = aligned(p.a, p.a_stride * ps, to) && aligned(p.b, p.b_stride * ps, to) &&
+              aligned(p.da, p.width * ps, to) && aligned(p.db, p.width * ps, to) && (p.width * ps) % to == 0;
+    if (p.one_plus && p.group == 1 && !p.p_vec) break;  // the ring moves both the same way
+    return vec;
+  }
+  p.p_vec = 0;
+  return (int)size;
 }
 
-cudaError_t launch_norm(const NormArgs& p, int x_type, bool backward, bool vec, cudaStream_t st) {
+cudaError_t launch_norm(const NormArgs& p, int x_type, bool backward, int vec, cudaStream_t st) {
   const bool wide = is_wide(p, x_type);
   cudaError_t e = x_type == LEWM_TYPE_F32    ? launch_norm_rows<float>(p, wide, backward, vec, st)
                   : x_type == LEWM_TYPE_BF16 ? launch_norm_rows<__nv_bfloat16>(p, wide, backward, vec, st)
@@ -205,10 +231,10 @@ using namespace lewm;
 extern "C" size_t lewm_norm_workspace(const lewm_norm_desc* desc) {
   NormArgs p;
   if (norm_args(desc, &p) != LEWM_OK || p.rows == 0) return 0;
-  cut_items(&p, desc->x_type, true, true);
-  const size_t vec = workspace_bytes(p);
-  cut_items(&p, desc->x_type, true, false);
-  return std::max(vec, workspace_bytes(p));  // whichever way the tensors lie
+  cut_items(&p, desc->x_type, true, 16);
+  const size_t bytes = workspace_bytes(p);
+  cut_items(&p, desc->x_type, true, 1);
+  return std::max(bytes, workspace_bytes(p));  // whichever way the tensors lie
 }
 
 extern "C" lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void* x, const void* a, const void* b,
@@ -229,7 +255,7 @@ extern "C" lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void*
   p.b = b;
   p.out = y;
   p.stats = stats;
-  const bool vec = vector_rows(&p, desc->x_type, false);
+  const int vec = vector_bytes(&p, desc->x_type, false);
   cut_items(&p, desc->x_type, false, vec);
   const cudaError_t e = launch_norm(p, desc->x_type, false, vec, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return norm_fail(LEWM_CUDA_ERROR, "norm forward launch: %s", cudaGetErrorString(e));
@@ -264,7 +290,7 @@ extern "C" lewm_status lewm_norm_backward(const lewm_norm_desc* desc, const void
   p.db = db;
   p.stats = const_cast<float*>(stats);
   p.ws = static_cast<float*>(workspace);
-  const bool vec = vector_rows(&p, desc->x_type, true);
+  const int vec = vector_bytes(&p, desc->x_type, true);
   cut_items(&p, desc->x_type, true, vec);
   if ((da || db) && workspace_bytes_given < workspace_bytes(p))
     return norm_fail(LEWM_INVALID_ARG, "workspace of %zu bytes, needs %zu", workspace_bytes_given, workspace_bytes(p));

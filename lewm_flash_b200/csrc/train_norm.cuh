@@ -17,17 +17,17 @@
 // store (mean and variance are two passes over registers), and sums over rows are kept in
 // registers by persistent blocks that own fixed columns, so x and dy are read once.
 //
-// Layout: a team of TPR threads holds one row, NV vectors of E elements per thread (16-byte
-// vectors where every row starts on 16 bytes, else single elements). In the backward that is at
+// Layout: a team of TPR threads holds one row, NV vectors of E elements per thread (vectors of 16, 8
+// or 4 bytes, whatever every row starts on, or single 16-bit elements). In the backward that is at
 // most 16 elements a thread: it then holds 16 gains and 32 sums, 128 registers at two 256-thread
 // blocks per SM. Rows of more than 32 KB take the looping kernels below.
 //
 // Rows arrive through a ring of 2 to 4 stages in shared memory, filled by cp.async one to
 // three rows ahead: registers alone kept 32 KB per SM on the way at best and none while a row
 // was being reduced, half of HBM's rate (131072 x 2048 bf16: forward 307 us, backward 404).
-// With 16-byte vectors each thread copies just what it reads itself, so the ring needs no
-// barrier; rows at odd addresses are copied by 16-byte pieces with 4-byte ends and read back
-// element by element after a team barrier.
+// With vectors each thread copies just what it reads itself, so the ring needs no barrier; rows
+// of odd 16-bit addresses (and odd float32 widths) are copied by 16-byte pieces with 4-byte ends and
+// read back element by element after a team barrier.
 //
 // Work is cut into items: a run of rows within one group. An item is a block's (its teams
 // interleave the rows and add up through shared memory), or a team's where there are many
@@ -300,8 +300,8 @@ __device__ __forceinline__ void cp_wait(int stages) {
 }
 
 // One stage of the ring for one tensor of element type P: a row of each team of the block.
-//   E > 1: vector i of a thread lies at [piece][i][thread] in 16-byte (or 8-byte) pieces; only
-//          that thread copies and reads it.
+//   E > 1: vector i of a thread lies at [piece][i][thread] in pieces of 16 bytes (8 or 4 where the
+//          vector is that small); only that thread copies and reads it.
 //   E = 1: a team's row lies in its slot at its address modulo 16; any thread copies any part.
 template <typename P, typename Tm>
 struct Stage {
@@ -326,7 +326,8 @@ struct Stage {
 #pragma unroll
           for (int k = 0; k < VB / PB; ++k) {
             if constexpr (PB == 16) cp_async16(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
-            else cp_async8(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
+            else if constexpr (PB == 8) cp_async8(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
+            else cp_async4(dst + (k * NV + i) * THREADS * PB, src + i * TPR * VB + k * PB);
           }
         }
       }
@@ -1073,7 +1074,7 @@ cudaError_t launch_ring(K kern, std::atomic<bool>* raised, int64_t grid, int thr
 // One pass of a tier, if the pass uses it: sets *e and returns true.
 template <typename T, typename P, int E, Pass PASS, int TPR, int N>
 bool launch_tier(const Tier& t, NormArgs p, cudaStream_t st, cudaError_t* e) {
-  constexpr int64_t MIN = min_width(TPR, N, PASS, E > 1);
+  constexpr int64_t MIN = min_width(TPR, N, PASS, E * sizeof(T) == 16);
   if constexpr (MIN > 0 && N % E == 0 && MIN * (int)sizeof(T) <= kMaxRowBytes) {
     if (t.tpr != TPR || t.n != N) return false;
     using Tm = Team<E, N / E, TPR, MIN>;
@@ -1105,7 +1106,7 @@ bool launch_tier(const Tier& t, NormArgs p, cudaStream_t st, cudaError_t* e) {
 
 template <typename T, typename P, int E, Pass PASS>
 bool launch_pass(const NormArgs& p, cudaStream_t st, cudaError_t* e) {
-  const Tier t = tier_of(p.width, PASS, dense_rows(p.rows, E > 1));
+  const Tier t = tier_of(p.width, PASS, dense_rows(p.rows, E * sizeof(T) == 16));
   return launch_tier<T, P, E, PASS, 8, 8>(t, p, st, e) || launch_tier<T, P, E, PASS, 8, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 8, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 16, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 16, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 8>(t, p, st, e) ||
@@ -1120,25 +1121,24 @@ bool launch_rows_mod(const NormArgs& p, bool backward, cudaStream_t st, cudaErro
 }
 
 template <typename T, int E>
-cudaError_t launch_width(const NormArgs& p, bool backward, cudaStream_t st) {
+cudaError_t launch_items(const NormArgs& p, bool backward, cudaStream_t st) {
   cudaError_t e = cudaErrorInvalidValue;
-  // A modulation row per row of x: the modulation in the ring, if two stages of it fit. bf16 beside
-  // fp16 goes without.
-  if (p.one_plus && p.group == 1) {
-    constexpr bool any = std::is_same<T, float>::value;
-    if (p.p_type == LEWM_TYPE_F32) {
-      if (launch_rows_mod<T, float, E>(p, backward, st, &e)) return e;
-    }
-    if constexpr (any || std::is_same<T, __nv_bfloat16>::value) {
-      if (p.p_type == LEWM_TYPE_BF16 && launch_rows_mod<T, __nv_bfloat16, E>(p, backward, st, &e)) return e;
-    }
-    if constexpr (any || std::is_same<T, __half>::value) {
-      if (p.p_type == LEWM_TYPE_F16 && launch_rows_mod<T, __half, E>(p, backward, st, &e)) return e;
-    }
-  }
   if (backward) launch_pass<T, T, E, BWD>(p, st, &e);
   else launch_pass<T, T, E, FWD>(p, st, &e);
   return e;
+}
+
+// A modulation row per row of x: the modulation in the ring, if two stages of it fit (false: no). bf16
+// beside fp16 goes without.
+template <typename T, int E>
+bool launch_modulated(const NormArgs& p, bool backward, cudaStream_t st, cudaError_t* e) {
+  constexpr bool any = std::is_same<T, float>::value;
+  if (p.p_type == LEWM_TYPE_F32) return launch_rows_mod<T, float, E>(p, backward, st, e);
+  if constexpr (any || std::is_same<T, __nv_bfloat16>::value)
+    if (p.p_type == LEWM_TYPE_BF16) return launch_rows_mod<T, __nv_bfloat16, E>(p, backward, st, e);
+  if constexpr (any || std::is_same<T, __half>::value)
+    if (p.p_type == LEWM_TYPE_F16) return launch_rows_mod<T, __half, E>(p, backward, st, e);
+  return false;
 }
 
 template <typename T, int E>
@@ -1157,9 +1157,20 @@ cudaError_t launch_wide(const NormArgs& p, bool backward, cudaStream_t st) {
 }  // namespace
 
 template <typename T>
-cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, bool vec, cudaStream_t st) {
-  if (wide) return vec ? launch_wide<T, 16 / sizeof(T)>(p, backward, st) : launch_wide<T, 1>(p, backward, st);
-  return vec ? launch_width<T, 16 / sizeof(T)>(p, backward, st) : launch_width<T, 1>(p, backward, st);
+cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, int vec, cudaStream_t st) {
+  constexpr int E16 = 16 / sizeof(T), E8 = 8 / sizeof(T);
+  if (wide) return vec == 16 ? launch_wide<T, E16>(p, backward, st) : launch_wide<T, 1>(p, backward, st);
+  if (p.one_plus && p.group == 1) {
+    cudaError_t e = cudaSuccess;
+    const bool done = vec == 16 ? launch_modulated<T, E16>(p, backward, st, &e)
+                                : launch_modulated<T, 1>(p, backward, st, &e);
+    if (done) return e;
+  }
+  if (vec == 16) return launch_items<T, E16>(p, backward, st);
+  if (vec == 8) return launch_items<T, E8>(p, backward, st);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 4) return launch_items<T, 2>(p, backward, st);
+  return launch_items<T, 1>(p, backward, st);
 }
 
 }  // namespace lewm

@@ -31,10 +31,10 @@ struct NormArgs {
 };
 
 // Launches one pass over rows of T (float, __nv_bfloat16, __half; a translation unit each) without the
-// final reduction of partial sums. `wide`: rows of more than kMaxRowBytes; `vec`: all rows and, with a
-// modulation row per row, the modulation start on their vectors.
+// final reduction of partial sums. `wide`: rows of more than kMaxRowBytes; `vec`: bytes of the vectors
+// that all rows start on (16, 8, 4 or one element's).
 template <typename T>
-cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, bool vec, cudaStream_t st);
+cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, int vec, cudaStream_t st);
 
 constexpr int kSms = 148;              // B200
 constexpr int kMaxRowBytes = 32768;    // widest row held by a block: 1024 threads x 16 16-bit elements

@@ -3,6 +3,6 @@
 
 namespace lewm {
 
-template cudaError_t launch_norm_rows<float>(const NormArgs& p, bool wide, bool backward, bool vec, cudaStream_t st);
+template cudaError_t launch_norm_rows<float>(const NormArgs& p, bool wide, bool backward, int vec, cudaStream_t st);
 
 }  // namespace lewm
