@@ -101,14 +101,14 @@ void cut_items(NormArgs* p, int x_type, bool backward, int vec) {
   const int64_t groups = p->rows / p->group;
   int64_t teams = 1;
   p->team_items = 0;
-  if (is_wide(*p, x_type)) {
+  if (is_wide(*p, x_type, backward)) {
     // Column blocks x items: split each group until the grid has about 4 blocks per SM.
     const int64_t cols = (p->width + 2047) / 2048;
     const int64_t want = (int64_t)kSms * 4 / std::max<int64_t>(1, cols * groups);
     p->split = (int)std::max<int64_t>(1, std::min<int64_t>(want, p->group));
   } else {
     const Pass pass = backward ? BWD : FWD;
-    const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec == 16));
+    const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec == 16), (int)type_size(x_type));
     teams = t.teams();
     // A team's items where a group has too few rows to keep a block's teams busy and there
     // are groups enough for every SM.
@@ -146,7 +146,7 @@ int vector_bytes(NormArgs* q, int x_type, bool backward) {
 }
 
 cudaError_t launch_norm(const NormArgs& p, int x_type, bool backward, int vec, cudaStream_t st) {
-  const bool wide = is_wide(p, x_type);
+  const bool wide = is_wide(p, x_type, backward);
   cudaError_t e = x_type == LEWM_TYPE_F32    ? launch_norm_rows<float>(p, wide, backward, vec, st)
                   : x_type == LEWM_TYPE_BF16 ? launch_norm_rows<__nv_bfloat16>(p, wide, backward, vec, st)
                                              : launch_norm_rows<__half>(p, wide, backward, vec, st);

@@ -13,7 +13,7 @@
 // Bound: bytes, 4 to 12 per element and pass. Many rows run at 91 to 102% of the rate of a plain copy
 // (131072 x 2048 bf16: forward 172 us, backward 261; 73881 x 1536 float32, groups of 8209 rows: 140 and
 // 203), at odd addresses at about 60%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
-// 35 and 52 us). A row therefore stays in registers from its only load to its only
+// 35 and 51 us). A row therefore stays in registers from its only load to its only
 // store (mean and variance are two passes over registers), and sums over rows are kept in
 // registers by persistent blocks that own fixed columns, so x and dy are read once.
 //
@@ -109,7 +109,15 @@ struct Tier {
 // threads have less to do one after the other (900 x 192 float32 forward 3.1 us, 4.8 in teams of 8), and
 // so do rows at odd addresses, whose single-element accesses are then 64 bytes wide.
 constexpr bool dense_rows(int64_t rows, bool vec) { return vec && rows >= 32 * kSms; }
-constexpr Tier tier_of(int64_t width, Pass pass, bool dense) {
+//
+// Wider rows take teams of a power of 2 with 16 values a thread, or
+//   24 in the forward of 16-bit rows, where half the team covers them: fewer idle lanes (49152 x 2720
+//      bf16 129 us with 16, 88 with 24; float32 rows, which are bound by DRAM, mostly lose: 73881 x 1536 from
+//      140 to 156);
+//   24 or 32 in the forward of more than 4096: two blocks per SM instead of one (16384 x 8192 bf16: 120
+//      and 85 us);
+//   12 in the backward where they cover the row (32768 x 1301 bf16 86 and 76 us).
+constexpr Tier tier_of(int64_t width, Pass pass, bool dense, int size) {
   if (width <= 64) return {8, 8};
   if (!dense) {
     if (width <= 256) return {32, 8};
@@ -119,26 +127,28 @@ constexpr Tier tier_of(int64_t width, Pass pass, bool dense) {
     if (width <= 256) return {16, 16};
     if (width <= 384 && pass != BWD) return {16, 24};
   }
-  // The forward keeps no sums: 32 values a thread leave two blocks per SM where 16 leave one.
-  if (!is_backward(pass) && width > 4096 && width <= 8192) return {256, 32};
   int tpr = 32;
   while (tpr * 16 < width) tpr *= 2;  // rows of at most kMaxRowBytes: tpr <= 1024
+  if (!is_backward(pass) && tpr >= 512) return {tpr / 2, width <= tpr * 12 ? 24 : 32};
+  if (pass == FWD && size == 2 && tpr > 32 && width <= tpr * 12) return {tpr / 2, 24};
+  if (pass == BWD && tpr > 32 && width <= tpr * 12) return {tpr, 12};
   return {tpr, 16};
 }
 // The narrowest row of a tier, 0 for one that the pass does not use. (The tiers that dense rows and
 // others share have the same narrowest row, or the lower one.)
-constexpr int64_t min_width_of(int tpr, int n, Pass pass, bool dense) {
-  const int64_t edges[] = {64, 128, 192, 256, 384, 512, 1024, 2048, 4096, 8192, 16384};
+constexpr int64_t min_width_of(int tpr, int n, Pass pass, bool dense, int size) {
+  const int64_t edges[] = {64,      128,  192,      256,  384,      512,  32 * 24,  1024,
+                           64 * 24, 2048, 128 * 24, 4096, 256 * 24, 8192, 512 * 24, 16384};
   int64_t before = 0;
   for (int64_t e : edges) {
-    const Tier t = tier_of(e, pass, dense);
+    const Tier t = tier_of(e, pass, dense, size);
     if (t.tpr == tpr && t.n == n) return before + 1;
     before = e;
   }
   return 0;
 }
-constexpr int64_t min_width(int tpr, int n, Pass pass, bool vec) {
-  const int64_t a = min_width_of(tpr, n, pass, false), b = vec ? min_width_of(tpr, n, pass, true) : 0;
+constexpr int64_t min_width(int tpr, int n, Pass pass, bool vec, int size) {
+  const int64_t a = min_width_of(tpr, n, pass, false, size), b = vec ? min_width_of(tpr, n, pass, true, size) : 0;
   return a == 0 ? b : b == 0 || a < b ? a : b;
 }
 
@@ -864,9 +874,12 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_BWD>) k_rowmod_bwd
   }
 }
 
-// ------------------------------------------------------------------ rows of more than kMaxRowBytes
+// ------------------------------------------------------------------ rows too wide for a block (is_wide)
 // A block per row, the row re-read (from L2) for each pass, in vectors of E elements.
-using Wide = Team<1, 2, 1024, 0>;
+// Threads of a block, 2048 on an SM: 256, 512 and 1024 took 35, 33 and 39 us forward (1000 x 20000 bf16) and
+// 414, 424 and 530 us backward (16384 x 10000 bf16).
+constexpr int kWideThreads = 512;
+using Wide = Team<1, 2, kWideThreads, 0>;
 
 // E elements of T at `q` as float32.
 template <typename T, int E>
@@ -903,7 +916,7 @@ __device__ __forceinline__ void load_params_f(const void* p, int type, int64_t a
 }
 
 template <typename T, int E>
-__global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
+__global__ void __launch_bounds__(kWideThreads, 2048 / kWideThreads) k_norm_fwd_wide(const NormArgs p) {
   griddep_wait();
   __shared__ float red[2][32];
   const float inv_n = 1.0f / p.width;
@@ -911,14 +924,14 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
     const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
     float s = 0.f, q = 0.f, f[E];
 #pragma unroll 4
-    for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
+    for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       load_f<T, E>(x + c, f);
 #pragma unroll
       for (int e = 0; e < E; ++e) s += f[e];
     }
     const float mu = Wide::sum(s, red[0]) / (float)p.width;
 #pragma unroll 4
-    for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
+    for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       load_f<T, E>(x + c, f);
 #pragma unroll
       for (int e = 0; e < E; ++e) q = fmaf(f[e] - mu, f[e] - mu, q);
@@ -932,7 +945,7 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
     T* y = static_cast<T*>(p.out) + r * p.width;
     const float plus = p.one_plus ? 1.f : 0.f;
 #pragma unroll 2
-    for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
+    for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       float a[E], b[E];
       load_f<T, E>(x + c, f);
       load_params_f<E>(p.a, p.p_type, g * p.a_stride + c, p.p_vec, 1.f, a);
@@ -945,7 +958,7 @@ __global__ void __launch_bounds__(1024) k_norm_fwd_wide(const NormArgs p) {
 }
 
 template <typename T, int E>
-__global__ void __launch_bounds__(1024) k_norm_dx_wide(const NormArgs p) {
+__global__ void __launch_bounds__(kWideThreads, 2048 / kWideThreads) k_norm_dx_wide(const NormArgs p) {
   griddep_wait();
   __shared__ float2 red[2][32];
   const float inv_n = 1.0f / p.width, plus = p.one_plus ? 1.f : 0.f;
@@ -968,7 +981,7 @@ __global__ void __launch_bounds__(1024) k_norm_dx_wide(const NormArgs p) {
       }
     };
 #pragma unroll 2
-    for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
+    for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       load(c);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -981,7 +994,7 @@ __global__ void __launch_bounds__(1024) k_norm_dx_wide(const NormArgs p) {
     const float m1 = s.x * inv_n, m2 = s.y * inv_n;
     T* o = static_cast<T*>(p.out) + r * p.width;
 #pragma unroll 2
-    for (int c = threadIdx.x * E; c < p.width; c += 1024 * E) {
+    for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       load(c);
 #pragma unroll
       for (int e = 0; e < E; ++e) d[e] = rs * (d[e] - m1 - z[e] * m2);
@@ -1030,7 +1043,12 @@ __global__ void __launch_bounds__(256) k_norm_sums_wide(const NormArgs p) {
 
 // ------------------------------------------------------------------ host side
 inline int64_t type_size(int type) { return type == LEWM_TYPE_F32 ? 4 : 2; }
-inline bool is_wide(const NormArgs& p, int x_type) { return p.width * type_size(x_type) > kMaxRowBytes; }
+// Rows for the looping kernels: too wide for a block's ring, or for its registers in the backward that
+// keeps sums (16384 x 10000 bf16: 555 us with 64 registers a thread and the rest spilled, 424 there).
+constexpr int64_t kMaxSumWidth = 8192;
+inline bool is_wide(const NormArgs& p, int x_type, bool backward) {
+  return p.width * type_size(x_type) > kMaxRowBytes || (backward && p.width > kMaxSumWidth);
+}
 
 // Rounds of loops over `rows` rows in steps of `step`. (No tensor that fits a GPU makes 2^31 rounds: a
 // step is a row for groups of a few, else a block's teams times the blocks that share the rows.)
@@ -1074,8 +1092,9 @@ cudaError_t launch_ring(K kern, std::atomic<bool>* raised, int64_t grid, int thr
 // One pass of a tier, if the pass uses it: sets *e and returns true.
 template <typename T, typename P, int E, Pass PASS, int TPR, int N>
 bool launch_tier(const Tier& t, NormArgs p, cudaStream_t st, cudaError_t* e) {
-  constexpr int64_t MIN = min_width(TPR, N, PASS, E * sizeof(T) == 16);
-  if constexpr (MIN > 0 && N % E == 0 && MIN * (int)sizeof(T) <= kMaxRowBytes) {
+  constexpr int64_t MIN = min_width(TPR, N, PASS, E * sizeof(T) == 16, sizeof(T));
+  if constexpr (MIN > 0 && N % E == 0 && MIN * (int)sizeof(T) <= kMaxRowBytes &&
+                !(PASS == BWD && MIN > kMaxSumWidth)) {
     if (t.tpr != TPR || t.n != N) return false;
     using Tm = Team<E, N / E, TPR, MIN>;
     static std::atomic<bool> raised[64];
@@ -1106,14 +1125,19 @@ bool launch_tier(const Tier& t, NormArgs p, cudaStream_t st, cudaError_t* e) {
 
 template <typename T, typename P, int E, Pass PASS>
 bool launch_pass(const NormArgs& p, cudaStream_t st, cudaError_t* e) {
-  const Tier t = tier_of(p.width, PASS, dense_rows(p.rows, E * sizeof(T) == 16));
+  const Tier t = tier_of(p.width, PASS, dense_rows(p.rows, E * sizeof(T) == 16), sizeof(T));
   return launch_tier<T, P, E, PASS, 8, 8>(t, p, st, e) || launch_tier<T, P, E, PASS, 8, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 8, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 16, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 16, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 8>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 32, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 128, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 16>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 256, 32>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 16>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 1024, 16>(t, p, st, e);
+         launch_tier<T, P, E, PASS, 256, 24>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 256, 32>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 24>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 64, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 128, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 512, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 32>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 1024, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 12>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 128, 12>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 12>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 512, 12>(t, p, st, e) || launch_tier<T, P, E, PASS, 1024, 12>(t, p, st, e);
 }
 template <typename T, typename P, int E>
 bool launch_rows_mod(const NormArgs& p, bool backward, cudaStream_t st, cudaError_t* e) {
@@ -1143,10 +1167,10 @@ bool launch_modulated(const NormArgs& p, bool backward, cudaStream_t st, cudaErr
 
 template <typename T, int E>
 cudaError_t launch_wide(const NormArgs& p, bool backward, cudaStream_t st) {
-  const dim3 rows_grid((unsigned)std::min<int64_t>(p.rows, 2 * kSms));
-  if (!backward) return launch_k(k_norm_fwd_wide<T, E>, rows_grid, dim3(1024), 0, st, p);
+  const dim3 rows_grid((unsigned)std::min<int64_t>(p.rows, kSms * (2048 / kWideThreads)));
+  if (!backward) return launch_k(k_norm_fwd_wide<T, E>, rows_grid, dim3(kWideThreads), 0, st, p);
   if (p.out) {
-    const cudaError_t e = launch_k(k_norm_dx_wide<T, E>, rows_grid, dim3(1024), 0, st, p);
+    const cudaError_t e = launch_k(k_norm_dx_wide<T, E>, rows_grid, dim3(kWideThreads), 0, st, p);
     if (e != cudaSuccess) return e;
   }
   if (!p.da && !p.db) return cudaSuccess;
@@ -1159,14 +1183,17 @@ cudaError_t launch_wide(const NormArgs& p, bool backward, cudaStream_t st) {
 template <typename T>
 cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, int vec, cudaStream_t st) {
   constexpr int E16 = 16 / sizeof(T), E8 = 8 / sizeof(T);
-  if (wide) return vec == 16 ? launch_wide<T, E16>(p, backward, st) : launch_wide<T, 1>(p, backward, st);
-  if (p.one_plus && p.group == 1) {
+  if (p.one_plus && p.group == 1 && p.width * (int)sizeof(T) <= kMaxRowBytes) {
     cudaError_t e = cudaSuccess;
     const bool done = vec == 16 ? launch_modulated<T, E16>(p, backward, st, &e)
                                 : launch_modulated<T, 1>(p, backward, st, &e);
     if (done) return e;
   }
-  if (vec == 16) return launch_items<T, E16>(p, backward, st);
+  if (wide) return vec == 16 ? launch_wide<T, E16>(p, backward, st) : launch_wide<T, 1>(p, backward, st);
+  // 12 values are no whole 16-byte vectors of 16-bit elements.
+  const bool halves = backward && tier_of(p.width, BWD, dense_rows(p.rows, vec == 16), sizeof(T)).n % E16 != 0;
+  if (vec == 16 && !halves) return launch_items<T, E16>(p, backward, st);
+  if (vec == 16) return launch_items<T, E8>(p, backward, st);
   if (vec == 8) return launch_items<T, E8>(p, backward, st);
   if constexpr (sizeof(T) == 2)
     if (vec == 4) return launch_items<T, 2>(p, backward, st);

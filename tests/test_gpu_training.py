@@ -63,7 +63,7 @@ def check_norm(x, a, b, eps, one_plus, group, y, dy, dx, da, db):
 
 SHAPES = [(1, 1), (1, 192), (3, 192), (2, 1), (5, 7), (33, 64), (900, 192), (257, 65), (130, 255), (131, 256), (70, 511),
           (65, 512), (40, 1011), (301, 1024), (37, 2048), (20, 4097), (9, 8192), (5, 16384), (3, 16385), (299, 20001),
-          (5000, 40), (2500, 770), (600, 154), (4800, 154), (333, 2274), (100, 5006), (700, 652), (50, 8190), (5000, 12)]
+          (5000, 40), (2500, 770), (600, 154), (4800, 154), (333, 2274), (100, 5006), (700, 652), (50, 8190), (5000, 12), (700, 10000), (90, 12301)]
 
 
 @pytest.mark.parametrize("types", TYPES, ids=TYPE_IDS)
@@ -87,7 +87,7 @@ def test_layer_norm_matches_64_bits(rows, width, types):
 @pytest.mark.parametrize("batch,tokens,width", [(1, 1, 192), (300, 3, 192), (7, 5, 33), (400, 1, 96), (1000, 5, 70),
                                                 (300, 17, 1024), (2, 5000, 96), (9, 700, 1536), (64, 257, 384),
                                                 (3, 2, 16385), (40, 15, 2050), (340, 41, 130),
-                                                (7, 300, 4100), (400, 6, 5006)])
+                                                (7, 300, 4100), (400, 6, 5006), (9, 40, 10008), (300, 1, 10001)])
 @pytest.mark.parametrize("shared", [False, True], ids=["per_token", "per_sequence"])
 def test_ada_layer_norm_matches_64_bits(batch, tokens, width, shared, types):
     dtype, ctype = types
