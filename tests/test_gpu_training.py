@@ -605,3 +605,91 @@ def test_cem_gd_steps_on_the_clipped_gradient():
     rt.sync()
     assert (got - by_hand(limit)).abs().max() <= 1e-5 * lr * steps
     assert torch.equal(refine(None), refine(math.inf)) and not torch.equal(got, refine(None))
+
+
+# ---------------------------------------------------------------------------- autograd's ways
+def test_graph_reused_and_released():
+    x, w = activation(300, 192, F32).requires_grad_(True), randn(192, seed=2).requires_grad_(True)
+    y = lf.layer_norm(x, w)
+    dy = randn(300, 192, seed=3)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    second = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, (x, w), dy)
+
+
+def test_one_graph_differentiated_on_two_streams_at_once():
+    x, w = activation(3000, 192, F32).requires_grad_(True), randn(192, seed=2).requires_grad_(True)
+    dy = [randn(3000, 192, seed=s) for s in (3, 4)]
+    y = lf.layer_norm(x, w)
+    want = [torch.autograd.grad(y, (x, w), d, retain_graph=True) for d in dy]
+    torch.cuda.synchronize()
+    got = []
+    for d in dy:
+        with torch.cuda.stream(torch.cuda.Stream(DEV)):
+            got.append(torch.autograd.grad(y, (x, w), d, retain_graph=True))
+    torch.cuda.synchronize()
+    for g, e in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(g, e))
+
+
+def test_threads():
+    """Passes and clips from several host threads, each on its own stream."""
+    import threading
+
+    x, w, dy = activation(900, 192, F32), randn(192, seed=2), randn(900, 192, seed=3)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+
+    def step():
+        return lf.clip_grads(torch.autograd.grad(lf.layer_norm(*leaves), leaves, dy), 0.5)
+
+    (want, norm), bad = step(), []
+    torch.cuda.synchronize()
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream(DEV)):
+            for _ in range(20):
+                got, n = step()
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(n, norm) and all(torch.equal(p, q) for p, q in zip(got, want))):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_inference_mode_and_accumulated_gradients():
+    x, w = activation(50, 192, BF16), randn(192, seed=2).requires_grad_(True)
+    with torch.inference_mode():
+        y = lf.layer_norm(x, w)
+        assert y.is_inference() and not y.requires_grad
+        g = torch.ones(100, device=DEV)
+        lf.clip_grads([g], 1.0, out=[g])
+        assert abs(float(g[0]) - 0.1) <= 1e-6
+    p = torch.nn.Parameter(randn(192, seed=3))
+    once = None
+    for k in (1, 2):
+        lf.layer_norm(activation(50, 192, F32), p).sum().backward()
+        once = p.grad.clone() if k == 1 else once
+    assert torch.equal(p.grad, once + once)
+
+
+def test_checkpointed_and_hooked_modules():
+    """Recomputed forwards (torch.utils.checkpoint) and module hooks see the routed modules."""
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(1)
+    model = TinyPredictor().to(DEV)
+    x, c = randn(10, 3, 64, seed=1).requires_grad_(True), randn(10, 3, 64, seed=2)
+    handle = lf.install_training_norms(model)
+    calls = []
+    model.norm.register_forward_hook(lambda m, i, o: calls.append(o.shape))
+    (want,) = torch.autograd.grad(model(x, c).square().sum(), x)
+    (got,) = torch.autograd.grad(checkpoint(model, x, c, use_reentrant=False).square().sum(), x)
+    assert torch.equal(got, want) and len(calls) >= 2  # the recomputation may stop before the last hook
+    handle.remove()
