@@ -45,6 +45,7 @@ int type_code(const Tensor& t) {
 void check_tensor(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(type_code(t) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
   TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor, got layout ", t.layout());
+  TORCH_CHECK_VALUE(!t.is_neg(), name, " is a lazily negated view: pass it through resolve_neg()");
 }
 
 void check_same_device(const char* name, const Tensor& t, const Tensor& x) {
@@ -297,7 +298,7 @@ Refs refs(const char* name, const py::list& list) {
 void check_list(const char* name, const Refs& ts) {
   for (size_t i = 0; i < ts.size(); ++i) {
     const Tensor& t = *ts[i];
-    if (type_code(t) < 0 || t.layout() != at::kStrided)
+    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg())
       check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
     TORCH_CHECK_VALUE(t.device() == ts[0]->device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
                       ts[0]->device(), ": one device per call");
@@ -408,7 +409,7 @@ std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, do
   const Refs out = refs("out", out_list);
   for (size_t i = 0; out_given && i < grads.size(); ++i) {
     const Tensor &g = *grads[i], &o = *out[i];
-    TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
+    TORCH_CHECK_VALUE(o.layout() == at::kStrided && !o.is_neg() && o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
                           o.device() == g.device(),
                       "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
     TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");

@@ -135,9 +135,10 @@ class B200TrainingNorms:
         for name, m in model.named_modules():
             if "forward" in m.__dict__:  # routed already, by this or another install
                 continue
-            if isinstance(m, torch.nn.LayerNorm) and len(m.normalized_shape) == 1:
+            if type(m).forward is torch.nn.LayerNorm.forward and len(m.normalized_shape) == 1:
                 m.forward = functools.partial(_layer_norm_forward, m)
-            elif (all(hasattr(m, n) for n in ("adaLN_modulation", "attn", "mlp"))
+            elif (type(m).__name__ == "ConditionalBlock"
+                  and all(hasattr(m, n) for n in ("adaLN_modulation", "attn", "mlp"))
                   and _plain_norm(getattr(m, "norm1", None)) and _plain_norm(getattr(m, "norm2", None))):
                 m.forward = functools.partial(_conditional_block_forward, m)
             else:
@@ -153,10 +154,11 @@ class B200TrainingNorms:
 
 
 def install_training_norms(model: torch.nn.Module) -> B200TrainingNorms:
-    """Route every ``nn.LayerNorm`` over the last dim and every AdaLN conditional block of ``model``
-    (reference ``lewm/module.py:38-53,56-111,131-187,217-240``: predictor, projector heads, and the ViT
-    encoder) through ``layer_norm`` and ``ada_layer_norm``, so that a training step of the world
-    model runs their forward and backward passes on the B200 kernels. Parameters, state dict and
+    """Route every ``nn.LayerNorm`` over the last dim (not subclasses with a forward of their own) and
+    every AdaLN ``ConditionalBlock`` of ``model`` (reference ``lewm/module.py:38-53,56-111,131-187,217-240``:
+    predictor, projector heads, and the ViT encoder) through ``layer_norm`` and ``ada_layer_norm``, so
+    that a training step of the world model runs their forward and backward passes on the B200
+    kernels. Parameters, state dict and
     autocast behaviour stay as they are: under autocast the norms run in float32 as torch's do.
     The model's inputs must be on a CUDA device."""
     return B200TrainingNorms(model)

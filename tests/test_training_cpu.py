@@ -21,6 +21,8 @@ z = torch.zeros
     (lambda: lf.layer_norm(z(3, 8, dtype=torch.float64)), "float32, bfloat16 or float16"),
     (lambda: lf.layer_norm(z(3, 8, dtype=torch.int32)), "float32, bfloat16 or float16"),
     (lambda: lf.layer_norm(z(3, 8).to_sparse()), "dense"),
+    (lambda: lf.layer_norm(torch._neg_view(z(3, 8))), "negated"),
+    (lambda: lf.grad_norm([torch._neg_view(z(3))]), "negated"),
     (lambda: lf.layer_norm(z(3, 8), z(7)), r"weight must be \(8,\)"),
     (lambda: lf.layer_norm(z(3, 8), z(8), z(1, 8)), r"bias must be \(8,\)"),
     (lambda: lf.layer_norm(z(3, 8), z(8), z(8).half()), "one type"),
@@ -237,9 +239,19 @@ def test_install_routes_norms_and_blocks_and_removes_them():
 
 
 def test_install_leaves_other_modules_alone():
+    class Scaled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Renamed(torch.nn.LayerNorm):
+        pass
+
+    class Block(ConditionalBlock):  # could do anything with its parts
+        pass
+
     model = torch.nn.Sequential(torch.nn.LayerNorm((3, 8)), torch.nn.Linear(8, 8), torch.nn.BatchNorm1d(8),
-                                torch.nn.LayerNorm(8))
-    assert lf.install_training_norms(model).modules == ["3"]
+                                torch.nn.LayerNorm(8), Scaled(8), Renamed(8), Block(8, 1, 8, 8))
+    assert lf.install_training_norms(model).modules == ["3", "5", "6.attn.norm", "6.mlp.0", "6.norm1", "6.norm2"]
 
 
 @pytest.mark.parametrize("value", [0.0, -1.0, math.nan])
