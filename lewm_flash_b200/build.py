@@ -75,7 +75,7 @@ def _build_ext(verbose: bool) -> None:
     for d in inc:
         cmd += ["-isystem", str(d)]
     cmd += ["-o", str(EXT) + ".tmp", *[str(CSRC / s) for s in EXT_SOURCES], "-L", str(PKG), "-llewm_b200",
-            "-L", str(tdir / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
+            "-L", str(tdir / "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda",
             "-Wl,-rpath,$ORIGIN"]
     _run(cmd, EXT, verbose)
 

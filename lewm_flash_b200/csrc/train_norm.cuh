@@ -11,8 +11,8 @@
 // share (a, b), with one group for layer norm, so one kernel each way serves both.
 //
 // Bound: bytes, 4 to 12 per element and pass. Many rows run at 91 to 102% of the rate of a plain copy
-// (131072 x 2048 bf16: forward 172 us, backward 261; 73881 x 1536 float32, groups of 8209 rows: 140 and
-// 203), at odd addresses at about 60%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
+// (131072 x 2048 bf16: forward 168 us, backward 261; 73881 x 1536 float32, groups of 8209 rows: 140 and
+// 206), at odd addresses at about 60%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
 // 35 and 51 us). A row therefore stays in registers from its only load to its only
 // store (mean and variance are two passes over registers), and sums over rows are kept in
 // registers by persistent blocks that own fixed columns, so x and dy are read once.
@@ -20,7 +20,8 @@
 // Layout: a team of TPR threads holds one row, NV vectors of E elements per thread (vectors of 16, 8
 // or 4 bytes, whatever every row starts on, or single 16-bit elements). In the backward that is at
 // most 16 elements a thread: it then holds 16 gains and 32 sums, 128 registers at two 256-thread
-// blocks per SM. Rows of more than 32 KB take the looping kernels below.
+// blocks per SM. Rows of more than 32 KB, and of more than 8192 values in the backward that keeps
+// sums, take the looping kernels below.
 //
 // Rows arrive through a ring of 2 to 4 stages in shared memory, filled by cp.async one to
 // three rows ahead: registers alone kept 32 KB per SM on the way at best and none while a row
@@ -1131,13 +1132,13 @@ bool launch_pass(const NormArgs& p, cudaStream_t st, cudaError_t* e) {
          launch_tier<T, P, E, PASS, 16, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 8>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 32, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 16>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 128, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 16>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 256, 24>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 256, 32>(t, p, st, e) || launch_tier<T, P, E, PASS, 32, 24>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 64, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 128, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 16>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 512, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 512, 32>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 1024, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 12>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 512, 16>(t, p, st, e) || launch_tier<T, P, E, PASS, 1024, 16>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 32, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 24>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 128, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 24>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 512, 24>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 32>(t, p, st, e) ||
+         launch_tier<T, P, E, PASS, 512, 32>(t, p, st, e) || launch_tier<T, P, E, PASS, 64, 12>(t, p, st, e) ||
          launch_tier<T, P, E, PASS, 128, 12>(t, p, st, e) || launch_tier<T, P, E, PASS, 256, 12>(t, p, st, e) ||
-         launch_tier<T, P, E, PASS, 512, 12>(t, p, st, e) || launch_tier<T, P, E, PASS, 1024, 12>(t, p, st, e);
+         launch_tier<T, P, E, PASS, 512, 12>(t, p, st, e);
 }
 template <typename T, typename P, int E>
 bool launch_rows_mod(const NormArgs& p, bool backward, cudaStream_t st, cudaError_t* e) {

@@ -37,6 +37,6 @@ template <typename T>
 cudaError_t launch_norm_rows(const NormArgs& p, bool wide, bool backward, int vec, cudaStream_t st);
 
 constexpr int kSms = 148;              // B200
-constexpr int kMaxRowBytes = 32768;    // widest row held by a block: 1024 threads x 16 16-bit elements
+constexpr int kMaxRowBytes = 32768;    // widest row held by a block: 512 threads x 32 16-bit elements
 
 }  // namespace lewm
