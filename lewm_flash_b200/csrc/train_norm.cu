@@ -96,6 +96,21 @@ int64_t best_split(int64_t groups, int64_t group, int64_t teams, int64_t full, b
   return best;
 }
 
+// Whether a team takes whole groups rather than a block (`split` items each): by the rounds of rows that
+// each way goes through, where an item of the block's costs about four rounds beside its rows, six in the
+// backward (it adds up its teams), and a team's four. A round of teams on rows far apart is dearer, by 6/5
+// with 16-bit rows and 5/3 with float32, measured over widths of 64 to 1024, groups of 3 to 60 rows and 300
+// to 19000 groups: 4700 groups of 3 x 192 bf16 forward and backward 37 and 57 us by blocks, 5.5 and 8.4 by
+// teams; 28 x 128: 30 and 63, 20 and 25; 2400 of 60 x 640: 80 and 129, 102 and 131.
+bool teams_pay(int64_t groups, int64_t group, int64_t teams, int64_t full, int64_t split, int size, bool backward) {
+  if (group > 64) return false;
+  const int64_t by_team = (groups + full * teams - 1) / (full * teams) * (group + 4);
+  const int64_t by_block = (groups * split + full - 1) / full *
+                               ((group + split * teams - 1) / (split * teams) + (backward ? 6 : 4)) +
+                           (backward && split > 1 ? 8 : 0);
+  return size == 2 ? by_team * 6 < by_block * 5 : by_team * 5 < by_block * 3;
+}
+
 // How rows are cut into items; the same function sizes the workspace.
 void cut_items(NormArgs* p, int x_type, bool backward, int vec) {
   const int64_t groups = p->rows / p->group;
@@ -110,10 +125,10 @@ void cut_items(NormArgs* p, int x_type, bool backward, int vec) {
     const Pass pass = backward ? BWD : FWD;
     const Tier t = tier_of(p->width, pass, dense_rows(p->rows, vec == 16), (int)type_size(x_type));
     teams = t.teams();
-    // A team's items where a group has too few rows to keep a block's teams busy and there
-    // are groups enough for every SM.
-    p->team_items = p->group < 2 * teams && groups >= kSms * teams;
-    p->split = p->team_items ? 1 : (int)best_split(groups, p->group, teams, (int64_t)kSms * bound_blocks(t.tpr, t.n, pass), backward);
+    const int64_t full = (int64_t)kSms * bound_blocks(t.tpr, t.n, pass);
+    const int64_t split = best_split(groups, p->group, teams, full, backward);
+    p->team_items = teams_pay(groups, p->group, teams, full, split, (int)type_size(x_type), backward);
+    p->split = p->team_items ? 1 : (int)split;
   }
   p->items = groups * p->split;
   set_loop(p, p->group, p->team_items ? 1 : p->split * teams);

@@ -101,6 +101,24 @@ def test_ada_layer_norm_matches_64_bits(batch, tokens, width, shared, types):
     check_norm(x, scale, shift, 1e-6, True, tokens if shared else 1, y.detach(), dy, dx, dscale, dshift)
 
 
+# Groups on both sides of the choice between a team and a block for each, a last block of teams that is not
+# full, and more groups than teams fit the GPU.
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, F32), (F16, F16)], ids=["f32", "bf16-f32", "f16"])
+@pytest.mark.parametrize("groups,group,width", [(37, 2, 64), (301, 3, 65), (1201, 4, 192), (4703, 3, 192), (4601, 28, 128),
+                                                (2400, 60, 96), (1203, 64, 40), (900, 65, 40), (19001, 2, 24),
+                                                (701, 7, 641), (1501, 2, 2048), (1201, 5, 1301), (613, 3, 4096),
+                                                (305, 2, 8192), (299, 2, 8200), (151, 3, 12000)])
+def test_ada_layer_norm_of_many_small_groups(groups, group, width, types):
+    dtype, ctype = types
+    x = activation(groups * group, width, dtype).view(groups, group, width).requires_grad_(True)
+    shift = randn(groups, 1, width, seed=3, scale=0.4, dtype=ctype).requires_grad_(True)
+    scale = randn(groups, 1, width, seed=5, scale=0.4, dtype=ctype).requires_grad_(True)
+    dy = randn(groups, group, width, seed=7, scale=0.1, dtype=dtype)
+    y = lf.ada_layer_norm(x, shift, scale)
+    dx, dshift, dscale = torch.autograd.grad(y, (x, shift, scale), dy)
+    check_norm(x, scale, shift, 1e-6, True, group, y.detach(), dy, dx, dscale, dshift)
+
+
 @pytest.mark.parametrize("shape,mod", [((4, 6, 3, 32), (4, 1, 1, 32)), ((4, 6, 3, 32), (4, 6, 1, 32)),
                                        ((4, 6, 3, 32), (32,)), ((4, 6, 3, 32), (1, 1, 1, 32)), ((6, 32), (6, 32)),
                                        ((1, 6, 32), (6, 32)), ((1, 32), (32,)), ((32,), (32,)), ((5, 1, 32), (5, 1, 32))])
