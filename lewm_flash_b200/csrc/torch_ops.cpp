@@ -146,7 +146,7 @@ struct NormBackward : public torch::autograd::Node {
 
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
-    Tensor dy = grads[0];
+    Tensor dy = std::move(grads[0]);
     const bool need_x = task_should_compute_output(0), need_a = has_a && task_should_compute_output(1),
                need_b = has_b && task_should_compute_output(2);
     if (!dy.defined() || !(need_x || need_a || need_b)) return out;
@@ -162,8 +162,10 @@ struct NormBackward : public torch::autograd::Node {
       at::NoGradGuard no_grad;
       const int64_t width = x_shape.back(), rows = x.numel() / width;
       if (need_x) out[0] = empty(x_shape, x.scalar_type(), x);
-      // A shift row per row of x: its gradient is dy.
-      const bool dy_is_db = need_b && group == 1 && rows > 0 && p_type == dy.scalar_type();
+      // A shift row per row of x: its gradient is dy, and may be dy's memory if nobody else holds that
+      // (the caller, another branch of the graph, a hook); else the kernel writes a copy.
+      const bool dy_is_db = need_b && group == 1 && rows > 0 && p_type == dy.scalar_type() && !twice &&
+                            dy.is_contiguous() && dy.use_count() == 1 && dy.has_storage() && dy.storage().use_count() == 1;
       if (rows == 0) {
         if (need_a) out[1] = empty(a_shape, p_type, x).zero_();
         if (need_b) out[2] = empty(b_shape, p_type, x).zero_();
@@ -182,7 +184,7 @@ struct NormBackward : public torch::autograd::Node {
                                           mut(out[2]), mut(ws), bytes, x.get_device(), stream_of(x)),
                        true);
         }
-        if (dy_is_db) out[2] = dy.detach().reshape(b_shape);
+        if (dy_is_db) out[2] = dy.sizes() == at::IntArrayRef(b_shape) ? std::move(dy) : dy.view(b_shape);
       }
     }
     if (twice) {

@@ -1,0 +1,71 @@
+"""Training operators on the GPU: the gradients' memory, and autograd's less usual callers."""
+
+import pytest
+import torch
+
+import lewm_flash_b200 as lf
+from tests.test_gpu_training import BF16, DEV, F32, activation, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------- whose memory a gradient is
+@pytest.mark.parametrize("shape", [(300, 3, 192), (6, 64), (40, 1030)])
+def test_gradients_of_a_shift_per_row_share_no_memory(shape):
+    """The shift's gradient is the output's gradient, in memory that nobody else holds: after two
+    accumulated passes each is the sum of two equal addends (exact), and the caller's own is as it was."""
+    x, scale = randn(*shape, seed=1), randn(*shape, seed=2, scale=0.3)
+    shifts = [randn(*shape, seed=s).requires_grad_(True) for s in (3, 4)]
+    g = randn(*shape, seed=5)
+    before = g.clone()
+    for _ in range(2):
+        (lf.ada_layer_norm(x, shifts[0], scale) + lf.ada_layer_norm(x, shifts[1], scale)).backward(g)
+    assert len({t.data_ptr() for t in (shifts[0].grad, shifts[1].grad, g)}) == 3
+    assert torch.equal(g, before)
+    assert torch.equal(shifts[0].grad, 2 * before) and torch.equal(shifts[1].grad, 2 * before)
+    norm = lf.clip_grad_norm_(shifts, 1.0)  # refuses gradients that overlap
+    assert norm > 1.0 and torch.equal(g, before)
+
+
+@pytest.mark.parametrize("retain", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_of_a_shift_per_row_from_an_operator_behind(dtype, retain):
+    """The output's gradient comes from an operator that keeps nothing of it, or, retained, is y.grad too."""
+    x, scale, k = (randn(50, 192, seed=s, dtype=dtype) for s in (1, 2, 3))
+    shift = randn(50, 192, seed=4, dtype=dtype).requires_grad_(True)
+    for n in (1, 2):
+        y = lf.ada_layer_norm(x, shift, scale)
+        if retain:
+            y.retain_grad()
+        (y * k).sum().backward()
+        assert torch.equal(shift.grad, n * k)
+        if retain:
+            assert torch.equal(y.grad, k) and y.grad.data_ptr() != shift.grad.data_ptr()
+    with torch.no_grad():
+        shift.grad.zero_()
+    assert k.any()
+
+
+def test_gradient_of_a_shift_per_row_seen_by_hooks():
+    """Hooks that keep the gradient they are shown keep it for themselves."""
+    x, scale, k = (randn(50, 192, seed=s) for s in (1, 2, 3))
+    shift = randn(50, 192, seed=4).requires_grad_(True)
+    y = lf.ada_layer_norm(x, shift, scale)
+    kept = []
+    y.register_hook(lambda g: kept.append(g))
+    y.grad_fn.register_hook(lambda gi, go: kept.append(go[0]))
+    shift.register_hook(lambda g: kept.append(g.clone()))
+    (y * k).sum().backward()
+    with torch.no_grad():
+        shift.grad.mul_(3.0)
+    assert len(kept) == 3 and all(torch.equal(g, k) for g in kept)
+
+
+def test_returned_gradient_of_a_shift_per_row_is_not_the_given_one():
+    x, scale = randn(20, 64, seed=1), randn(20, 64, seed=2)
+    shift, g = randn(20, 64, seed=3).requires_grad_(True), randn(20, 64, seed=4)
+    (d,) = torch.autograd.grad(lf.ada_layer_norm(x, shift, scale), shift, g)
+    assert torch.equal(d, g) and d.data_ptr() != g.data_ptr()
+    before = g.clone()
+    lf.clip_grads([d], 0.1, out=[d])
+    assert torch.equal(g, before)
