@@ -7,6 +7,7 @@
 // Python autograd.Function and ctypes 140 us, through this module's autograd node 62 us (45 of
 // them the autograd engine's own); a forward pass alone 15 and 4 us; a clip of 523 tensors, with
 // its checks, 677 and 48 us.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -43,10 +44,21 @@ int type_code(const Tensor& t) {
   }
 }
 
+// A tangent (torch.autograd.forward_ad) that the kernels would drop.
+bool has_tangent(const Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::isFwGradDefined(t);
+}
+
+void check_no_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " has a tangent: the B200 training operators have no "
+                              "forward-mode derivative");
+}
+
 void check_tensor(const char* name, const Tensor& t) {
   TORCH_CHECK_VALUE(type_code(t) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
   TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor, got layout ", t.layout());
   TORCH_CHECK_VALUE(!t.is_neg(), name, " is a lazily negated view: pass it through resolve_neg()");
+  check_no_tangent(name, t);
 }
 
 void check_same_device(const char* name, const Tensor& t, const Tensor& x) {
@@ -150,6 +162,7 @@ struct NormBackward : public torch::autograd::Node {
     const bool need_x = task_should_compute_output(0), need_a = has_a && task_should_compute_output(1),
                need_b = has_b && task_should_compute_output(2);
     if (!dy.defined() || !(need_x || need_a || need_b)) return out;
+    check_no_tangent("the output's gradient", dy);
     Tensor x, a, stats;
     {
       std::lock_guard<std::mutex> lock(mutex_);
@@ -306,7 +319,7 @@ Refs refs(const char* name, const py::list& list) {
 void check_list(const char* name, const Refs& ts) {
   for (size_t i = 0; i < ts.size(); ++i) {
     const Tensor& t = *ts[i];
-    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg())
+    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg() || has_tangent(t))
       check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
     TORCH_CHECK_VALUE(t.device() == ts[0]->device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
                       ts[0]->device(), ": one device per call");
@@ -420,6 +433,7 @@ std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, do
                           o.device() == g.device(),
                       "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
     TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");
+    if (has_tangent(o)) check_no_tangent(("out[" + std::to_string(i) + "]").c_str(), o);
   }
   std::vector<Tensor> copies;
   Tensor norm = clip(dense(grads, &copies), &out, limit, kind, Tensor());

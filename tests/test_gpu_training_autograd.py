@@ -69,3 +69,29 @@ def test_returned_gradient_of_a_shift_per_row_is_not_the_given_one():
     before = g.clone()
     lf.clip_grads([d], 0.1, out=[d])
     assert torch.equal(g, before)
+
+
+# ---------------------------------------------------------------------------- forward mode
+def test_forward_mode_through_a_backward_pass_is_refused():
+    """A tangent on the output's gradient (forward over reverse) would be dropped."""
+    import torch.autograd.forward_ad as fwd
+
+    x = randn(4, 32).requires_grad_(True)
+    y = lf.layer_norm(x)
+    with fwd.dual_level():
+        dy = fwd.make_dual(randn(4, 32, seed=1), randn(4, 32, seed=2))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, dy)
+
+
+def test_forward_mode_is_refused_on_the_gpu():
+    import torch.autograd.forward_ad as fwd
+
+    x, w = randn(4, 32), randn(32)
+    with fwd.dual_level():
+        for args in ((fwd.make_dual(x, x), w), (x, fwd.make_dual(w, w))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                lf.layer_norm(*args)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            lf.grad_norm([x, fwd.make_dual(x, x)])
+        lf.layer_norm(x, w)  # nothing dual: as ever

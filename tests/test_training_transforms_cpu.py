@@ -1,0 +1,42 @@
+"""Training operators, no GPU: callers that the kernels would answer wrongly are refused by name, before
+anything else is looked at."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import lewm_flash_b200 as lf
+
+z = torch.zeros
+
+
+# ---------------------------------------------------------------------------- forward mode
+@pytest.mark.parametrize("call", [
+    lambda d: lf.layer_norm(d(3, 8)),
+    lambda d: lf.layer_norm(z(3, 8), d(8)),
+    lambda d: lf.layer_norm(z(3, 8), z(8), d(8)),
+    lambda d: lf.ada_layer_norm(d(3, 8), z(8), z(8)),
+    lambda d: lf.ada_layer_norm(z(3, 8), d(8), z(8)),
+    lambda d: lf.ada_layer_norm(z(3, 8), z(8), d(8)),
+    lambda d: lf.grad_norm([z(3), d(3)]),
+    lambda d: lf.clip_grads([d(3)], 1.0),
+    lambda d: lf.clip_grads([z(3)], 1.0, out=[d(3)]),
+])
+def test_forward_mode_is_refused(call):
+    with fwd.dual_level():
+        def dual(*shape):
+            return fwd.make_dual(z(*shape), torch.ones(*shape))
+
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):  # has tangents all the same
+            call(dual)
+        with pytest.raises(ValueError, match="need a CUDA device"):
+            call(z)
+
+
+def test_forward_mode_of_a_routed_model_is_refused():
+    model = torch.nn.Sequential(torch.nn.LayerNorm(8))
+    lf.install_training_norms(model)
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        model(fwd.make_dual(z(3, 8), z(3, 8)))
