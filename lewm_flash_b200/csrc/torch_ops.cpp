@@ -8,6 +8,8 @@
 // them the autograd engine's own); a forward pass alone 15 and 4 us; a clip of 523 tensors, with
 // its checks, 677 and 48 us.
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -17,6 +19,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
 
 #include <algorithm>
@@ -42,6 +45,20 @@ int type_code(const Tensor& t) {
     case at::kHalf: return LEWM_TYPE_F16;
     default: return -1;
   }
+}
+
+// A tracer (torch.jit.trace, make_fx, torch.export) records what goes through torch's dispatcher. It
+// does not see these calls and would take their outputs for constants.
+void check_no_tracer() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  const bool tracing = at::tracer::impl::is_dispatch_enabled() ||
+                       c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                       TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value() ||
+                       TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL).has_value() ||
+                       TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE).has_value();
+  TORCH_CHECK_NOT_IMPLEMENTED(!tracing, "the B200 training operators cannot be traced: trace the model without them "
+                              "(install_training_norms(...).remove())");
 }
 
 // A tangent (torch.autograd.forward_ad) that the kernels would drop.
@@ -162,6 +179,7 @@ struct NormBackward : public torch::autograd::Node {
     const bool need_x = task_should_compute_output(0), need_a = has_a && task_should_compute_output(1),
                need_b = has_b && task_should_compute_output(2);
     if (!dy.defined() || !(need_x || need_a || need_b)) return out;
+    check_no_tracer();
     check_no_tangent("the output's gradient", dy);
     Tensor x, a, stats;
     {
@@ -247,6 +265,7 @@ Tensor norm(const Tensor& x, const Tensor& a, const Tensor& b, float eps, int64_
 }
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+  check_no_tracer();
   check_tensor("x", x);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last dim of at least 1, got shape ", x.sizes());
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
@@ -265,6 +284,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
 }
 
 Tensor ada_layer_norm(const Tensor& x, const Tensor& shift, const Tensor& scale, double eps) {
+  check_no_tracer();
   check_tensor("x", x);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "x must have a last dim of at least 1, got shape ", x.sizes());
   check_tensor("shift", shift);
@@ -402,6 +422,7 @@ void bump(const Tensor& t) {
 }
 
 Tensor grad_norm(const py::list& list, double norm_type) {
+  check_no_tracer();
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   const Refs grads = refs("grads", list);
@@ -413,6 +434,7 @@ Tensor grad_norm(const py::list& list, double norm_type) {
 
 std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, double norm_type,
                                        const std::optional<py::list>& out_given) {
+  check_no_tracer();
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   const float limit = check_max_norm(max_norm);
@@ -443,6 +465,7 @@ std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, do
 }
 
 Tensor clip_in_place(const py::list& list, double max_norm, double norm_type, bool error_if_nonfinite) {
+  check_no_tracer();
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   const float limit = check_max_norm(max_norm);

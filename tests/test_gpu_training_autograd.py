@@ -95,3 +95,27 @@ def test_forward_mode_is_refused_on_the_gpu():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             lf.grad_norm([x, fwd.make_dual(x, x)])
         lf.layer_norm(x, w)  # nothing dual: as ever
+
+
+# ---------------------------------------------------------------------------- tracers
+def test_tracing_is_refused_on_the_gpu():
+    """A tracer does not see the kernels and would record their output as a constant."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, w = randn(4, 32), randn(32)
+    for call in (lambda t: lf.layer_norm(t, w), lambda t: lf.ada_layer_norm(t, w, w), lambda t: lf.grad_norm([t]),
+                 lambda t: lf.clip_grads([t], 0.1)[0][0]):
+        for trace in (lambda f: torch.jit.trace(f, (x,), check_trace=False), lambda f: make_fx(f)(x),
+                      lambda f: make_fx(f, tracing_mode="fake")(x), lambda f: make_fx(f, pre_dispatch=True)(x)):
+            with pytest.raises(NotImplementedError, match="trac"):
+                trace(call)
+        call(x)  # the tracer is gone
+
+
+def test_tracing_a_backward_pass_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = randn(4, 32).requires_grad_(True)
+    y = lf.layer_norm(x)
+    with pytest.raises(NotImplementedError, match="trac"):
+        make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0])(randn(4, 32, seed=1))

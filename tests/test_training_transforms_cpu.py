@@ -4,6 +4,7 @@ anything else is looked at."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import lewm_flash_b200 as lf
 
@@ -40,3 +41,21 @@ def test_forward_mode_of_a_routed_model_is_refused():
     lf.install_training_norms(model)
     with fwd.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         model(fwd.make_dual(z(3, 8), z(3, 8)))
+
+
+# ---------------------------------------------------------------------------- tracers
+@pytest.mark.parametrize("trace", [
+    lambda f, x: torch.jit.trace(f, (x,), check_trace=False),
+    lambda f, x: make_fx(f)(x),
+    lambda f, x: make_fx(f, tracing_mode="fake")(x),
+    lambda f, x: make_fx(f, tracing_mode="symbolic")(x),
+    lambda f, x: make_fx(f, pre_dispatch=True)(x),
+], ids=["jit", "make_fx", "fake", "symbolic", "pre_dispatch"])
+@pytest.mark.parametrize("call", [lambda x: lf.layer_norm(x), lambda x: lf.ada_layer_norm(x, z(8), z(8)),
+                                  lambda x: lf.grad_norm([x]), lambda x: lf.clip_grads([x], 1.0)[1],
+                                  lambda x: x + lf.layer_norm(z(8))])
+def test_tracing_is_refused(call, trace):
+    with pytest.raises(NotImplementedError, match="cannot be traced"):
+        trace(call, z(3, 8))
+    with pytest.raises(ValueError, match="need a CUDA device"):
+        call(z(3, 8))
