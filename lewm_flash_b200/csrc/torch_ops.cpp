@@ -191,6 +191,7 @@ struct NormBackward : public torch::autograd::Node {
     const bool twice = at::GradMode::is_enabled();  // create_graph: a second pass would need our derivative
     {
       at::NoGradGuard no_grad;
+      if (dy.is_neg()) dy = dy.resolve_neg();
       const int64_t width = x_shape.back(), rows = x.numel() / width;
       if (need_x) out[0] = empty(x_shape, x.scalar_type(), x);
       // A shift row per row of x: its gradient is dy, and may be dy's memory if nobody else holds that

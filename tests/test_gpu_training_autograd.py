@@ -119,3 +119,20 @@ def test_tracing_a_backward_pass_is_refused():
     y = lf.layer_norm(x)
     with pytest.raises(NotImplementedError, match="trac"):
         make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0])(randn(4, 32, seed=1))
+
+
+# ---------------------------------------------------------------------------- lazily negated gradients
+@pytest.mark.parametrize("rows,width", [(50, 1), (50, 192), (9, 20000)])
+def test_lazily_negated_output_gradient(rows, width):
+    x, w, b = randn(rows, width, seed=1), randn(width, seed=2), randn(width, seed=3)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dy = randn(rows, width, seed=4)
+    y = lf.layer_norm(*leaves)
+    want = torch.autograd.grad(y, leaves, -dy, retain_graph=True)
+    got = torch.autograd.grad(y, leaves, torch._neg_view(dy))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    shift, scale = (randn(rows, width, seed=s).requires_grad_(True) for s in (5, 6))
+    y = lf.ada_layer_norm(x, shift, scale)
+    want = torch.autograd.grad(y, (x, shift, scale), -dy, retain_graph=True)
+    got = torch.autograd.grad(y, (x, shift, scale), torch._neg_view(dy))
+    assert all(torch.equal(p, q) and not p.is_neg() for p, q in zip(got, want))
