@@ -48,6 +48,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -183,6 +184,26 @@ struct Team {
       for (int i = 0; i < TPR / 32; ++i) v += red[w0 + i];
     }
     return v;
+  }
+  // The sum over a team of more than 8 warps and what its last addition lost: exact where the sums of
+  // 8 warps are.
+  static __device__ __forceinline__ float2 sum_and_rest(float v, float* red) {
+    constexpr int WARPS = TPR / 32;
+    static_assert(WARPS > 8 && WARPS <= 16, "two runs of warps");
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warp = threadIdx.x >> 5, w0 = team() * WARPS;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    barrier();
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a += red[w0 + i];
+      if (8 + i < WARPS) b += red[w0 + 8 + i];
+    }
+    // The rounding error of a + b (Knuth's TwoSum).
+    const float s = a + b, t = s - a;
+    return make_float2(s, (a - (s - t)) + (b - t));
   }
   static __device__ __forceinline__ float2 sum2(float2 v, float2* red) {
     constexpr int W = TPR < 32 ? TPR : 32;
@@ -488,35 +509,72 @@ __device__ __forceinline__ void load_offset(const NormArgs& p, int64_t g, F2* b)
 }
 
 // ------------------------------------------------------------------ forward
-// x - mu in place of the team's values x (0 beyond the row), mu and rs. The mean is divided, not
-// multiplied by 1 / n: that of a constant row (padding) is then the constant, and z is 0, where one
-// rounding of mu would come out as rs = 1 / sqrt(eps) times itself.
-template <typename Tm>
-__device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float (*red)[32]) {
+// The variance from the sums q of c^2 and s of c, and d = s / n: mean(c^2) - d^2. q of infinity stays.
+__device__ __forceinline__ float variance(float q, float s, float d, float inv_n) {
+  return (q <= FLT_MAX ? fmaxf(fmaf(-s, d, q), 0.f) : q) * inv_n;
+}
+
+// x - mean in place of the team's values x (0 beyond the row), mean and rs. An error of the mean comes out up
+// to 1 / sqrt(eps) times as large, so that of float32 rows, whose sum is rounded, is taken in two steps:
+// c = x - mu with the rounded mean mu, then what is left, d = mean(c), comes off too (and off the variance,
+// mean(c^2) - d^2). In one step a constant row (padding) of 1234.567 gave z of 0.1 instead of 0. The sum of a
+// constant row c of 16-bit values is exact, but for fp16 (11 bits) beyond 8192 of them: the last addition's
+// error is kept there. n c / n is c then, and z of a constant row 0. One step and two: 73881 x 1536 float32
+// 140 and 141 us, 57600 x 192 16.4 and 16.5, 32768 x 2720 120 and 121; 16384 x 16384 fp16 without and with
+// the error 193 and 193.
+template <typename T, typename Tm>
+__device__ __forceinline__ float2 row_stats(F2* f, int width, float inv_n, float eps, float2 (*red)[32]) {
   constexpr int E = Tm::E, TPR = Tm::TPR;
+  constexpr bool TWO_STEPS = sizeof(T) == 4;
+  constexpr bool REST = std::is_same<T, __half>::value && TPR * Tm::N > 8192;
   F2 s = f2(0.f), q = f2(0.f);
 #pragma unroll
   for (int k = 0; k < Tm::H; ++k) s = s + f[k];
-  const float mu = Tm::sum(both(s), red[0]) / (float)width;
+  float* const red0 = reinterpret_cast<float*>(red[0]);
+  float mu;
+  if constexpr (TWO_STEPS) {
+    mu = Tm::sum(both(s), red0) * inv_n;
+  } else if constexpr (REST) {
+    const float2 sum = Tm::sum_and_rest(both(s), red0);
+    mu = sum.x / (float)width;
+    mu = fmaf(fmaf(-mu, (float)width, sum.x) + sum.y, inv_n, mu);
+  } else {
+    mu = Tm::sum(both(s), red0) / (float)width;
+  }
   const F2 nm = f2(-mu);
+  s = f2(0.f);
 #pragma unroll
   for (int k = 0; k < Tm::H; ++k) {
     f[k] = f[k] + nm;
     if constexpr (E > 1) {
       const int i = k / (E / 2);
-      if (i < Tm::SURE || Tm::lane() + i * TPR < width / E) q = fma2(f[k], f[k], q);
+      if (i < Tm::SURE || Tm::lane() + i * TPR < width / E) {
+        q = fma2(f[k], f[k], q);
+        if constexpr (TWO_STEPS) s = s + f[k];
+      }
     } else {
       const int i = 2 * k;
-      if (i + 1 < Tm::SURE) {
-        q = fma2(f[k], f[k], q);
-      } else {
-        const float2 v = split(f[k]);
-        const F2 c = f2(Tm::lane() + i * TPR < width ? v.x : 0.f, Tm::lane() + (i + 1) * TPR < width ? v.y : 0.f);
-        q = fma2(c, c, q);
+      F2 c = f[k];
+      if (i + 1 >= Tm::SURE) {
+        const float2 v = split(c);
+        c = f2(Tm::lane() + i * TPR < width ? v.x : 0.f, Tm::lane() + (i + 1) * TPR < width ? v.y : 0.f);
       }
+      q = fma2(c, c, q);
+      if constexpr (TWO_STEPS) s = s + c;
     }
   }
-  const float var = Tm::sum(both(q), red[1]) * inv_n;
+  float var;
+  if constexpr (TWO_STEPS) {
+    const float2 qs = Tm::sum2(make_float2(both(q), both(s)), red[1]);
+    const float d = qs.y / (float)width;
+    var = variance(qs.x, qs.y, d, inv_n);
+    mu += d;
+    const F2 nd = f2(-d);
+#pragma unroll
+    for (int k = 0; k < Tm::H; ++k) f[k] = f[k] + nd;
+  } else {
+    var = Tm::sum(both(q), reinterpret_cast<float*>(red[1])) * inv_n;
+  }
   return make_float2(mu, 1.0f / sqrtf(var + eps));
 }
 
@@ -526,7 +584,7 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, FWD>) k_norm_fwd(const
   using St = Stage<T, Tm>;
   constexpr int H = Tm::H;
   extern __shared__ __align__(16) char ring[];
-  __shared__ float red[2][32];
+  __shared__ float2 red[2][32];
   const float inv_n = 1.0f / p.width;
   const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * St::BYTES;
   const int64_t per_block = p.team_items ? Tm::TEAMS : 1;
@@ -563,7 +621,7 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, FWD>) k_norm_fwd(const
         for (int h = 0; h < H; ++h) f[h] = f2(0.f);
       }
       out = out + St::BYTES == ring_end ? ring0 : out + St::BYTES;
-      const float2 ms = row_stats<Tm>(f, p.width, inv_n, p.eps, red);
+      const float2 ms = row_stats<T, Tm>(f, p.width, inv_n, p.eps, red);
       if (left > 0) {
         if (p.stats && Tm::lane() == 0) {
           p.stats[r] = ms.x;
@@ -591,7 +649,7 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_FWD>) k_rowmod_fwd
   using Sp = Stage<P, Tm>;
   constexpr int H = Tm::H, BYTES = St::BYTES + 2 * Sp::BYTES;
   extern __shared__ __align__(16) char ring[];
-  __shared__ float red[2][32];
+  __shared__ float2 red[2][32];
   const float inv_n = 1.0f / p.width;
   const uint32_t ring0 = smem_u32(ring), ring_end = ring0 + p.stages * BYTES;
   const int64_t first = (int64_t)blockIdx.x * Tm::TEAMS + Tm::team(), step = (int64_t)gridDim.x * Tm::TEAMS;
@@ -629,7 +687,7 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_FWD>) k_rowmod_fwd
 #pragma unroll
       for (int h = 0; h < H; ++h) f[h] = f2(0.f);
     }
-    const float2 ms = row_stats<Tm>(f, p.width, inv_n, p.eps, red);
+    const float2 ms = row_stats<T, Tm>(f, p.width, inv_n, p.eps, red);
     if (left > 0) {
       if (p.stats && Tm::lane() == 0) {
         p.stats[r] = ms.x;
@@ -919,7 +977,7 @@ __device__ __forceinline__ void load_params_f(const void* p, int type, int64_t a
 template <typename T, int E>
 __global__ void __launch_bounds__(kWideThreads, 2048 / kWideThreads) k_norm_fwd_wide(const NormArgs p) {
   griddep_wait();
-  __shared__ float red[2][32];
+  __shared__ float2 red[2][32];
   const float inv_n = 1.0f / p.width;
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(p.x) + r * p.x_stride;
@@ -930,16 +988,24 @@ __global__ void __launch_bounds__(kWideThreads, 2048 / kWideThreads) k_norm_fwd_
 #pragma unroll
       for (int e = 0; e < E; ++e) s += f[e];
     }
-    const float mu = Wide::sum(s, red[0]) / (float)p.width;
+    const float mu = Wide::sum(s, reinterpret_cast<float*>(red[0])) * inv_n;
+    s = 0.f;
 #pragma unroll 4
     for (int c = threadIdx.x * E; c < p.width; c += kWideThreads * E) {
       load_f<T, E>(x + c, f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) q = fmaf(f[e] - mu, f[e] - mu, q);
+      for (int e = 0; e < E; ++e) {
+        const float c = f[e] - mu;
+        q = fmaf(c, c, q);
+        s += c;
+      }
     }
-    const float rs = 1.0f / sqrtf(Wide::sum(q, red[1]) * inv_n + p.eps);
+    // The mean in two steps, as row_stats takes it.
+    const float2 qs = Wide::sum2(make_float2(q, s), red[1]);
+    const float d = qs.y / (float)p.width;
+    const float rs = 1.0f / sqrtf(variance(qs.x, qs.y, d, inv_n) + p.eps);
     if (p.stats && threadIdx.x == 0) {
-      p.stats[r] = mu;
+      p.stats[r] = mu + d;
       p.stats[p.rows + r] = rs;
     }
     const int64_t g = r / p.group;
@@ -952,7 +1018,7 @@ __global__ void __launch_bounds__(kWideThreads, 2048 / kWideThreads) k_norm_fwd_
       load_params_f<E>(p.a, p.p_type, g * p.a_stride + c, p.p_vec, 1.f, a);
       load_params_f<E>(p.b, p.p_type, g * p.b_stride + c, p.p_vec, 0.f, b);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = fmaf((f[e] - mu) * rs, a[e] + plus, b[e]);
+      for (int e = 0; e < E; ++e) f[e] = fmaf((f[e] - mu - d) * rs, a[e] + plus, b[e]);
       store_f<T, E>(y + c, f);
     }
   }
