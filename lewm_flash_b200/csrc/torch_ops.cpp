@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <cmath>
 #include <limits>
+#include <numeric>
 #include <optional>
 #include <vector>
 
@@ -369,6 +370,76 @@ bool overlap(const std::vector<int64_t>& src, const std::vector<int64_t>& dst, c
   return false;
 }
 
+// The bytes of a strided tensor: runs of `run` bytes from `base` on, at all sums of multiples of the
+// strides, the largest first. Each stride reaches past all that lies under it, so no two elements meet.
+struct Region {
+  struct Dim {
+    int64_t stride, size, inner;  // bytes; inner: from first to last byte of what lies under the dim
+  };
+  int64_t base = 0, run = 0, span = 0;
+  std::vector<Dim> dims;
+  bool own_overlap = false;
+
+  explicit Region(const Tensor& t) : base(reinterpret_cast<int64_t>(t.const_data_ptr())) {
+    if (t.numel() == 0) return;
+    std::vector<std::pair<int64_t, int64_t>> by_stride;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1) by_stride.emplace_back(t.stride(d) * t.element_size(), t.size(d));
+    std::sort(by_stride.begin(), by_stride.end());
+    run = span = t.element_size();
+    for (const auto& [stride, size] : by_stride) {
+      own_overlap |= stride < span;
+      if (dims.empty() && stride == run) run = span = run * size;
+      else dims.push_back({stride, size, span}), span += (size - 1) * stride;
+    }
+    std::reverse(dims.begin(), dims.end());
+  }
+};
+
+// Whether the parts of a and b from their dims i and j on, at x and y, share a byte. Gives up with true
+// after `steps` splits.
+bool meet(const Region& a, size_t i, int64_t x, const Region& b, size_t j, int64_t y, int64_t* steps) {
+  const bool split_a = i < a.dims.size(), split_b = j < b.dims.size();
+  const int64_t span_a = split_a ? a.dims[i].inner + (a.dims[i].size - 1) * a.dims[i].stride : a.run;
+  const int64_t span_b = split_b ? b.dims[j].inner + (b.dims[j].size - 1) * b.dims[j].stride : b.run;
+  if (x >= y + span_b || y >= x + span_a) return false;
+  if (!split_a && !split_b) return true;
+  if (--*steps < 0) return true;
+  // Runs that are apart modulo a divisor of all strides are apart: columns of one buffer.
+  int64_t g = 0;
+  for (size_t k = i; k < a.dims.size(); ++k) g = std::gcd(g, a.dims[k].stride);
+  for (size_t k = j; k < b.dims.size(); ++k) g = std::gcd(g, b.dims[k].stride);
+  const int64_t from = ((y - x) % g + g) % g;  // of b's run behind a's, round the circle
+  if (from >= a.run && from + b.run <= g) return false;
+  // Split the one that spans more; only its parts near the other one.
+  if (!split_a || (split_b && span_b > span_a)) return meet(b, j, y, a, i, x, steps);
+  const Region::Dim& d = a.dims[i];
+  const int64_t after = y - x - d.inner;  // a part that starts at or before it ends before b begins
+  const int64_t first = after < 0 ? 0 : after / d.stride + 1, last = std::min(d.size - 1, (y + span_b - 1 - x) / d.stride);
+  for (int64_t k = first; k <= last; ++k)
+    if (meet(a, i + 1, x + k * d.stride, b, j, y, steps)) return true;
+  return false;
+}
+
+// Refuses gradients, some of them strided, that share memory with each other or within themselves.
+void check_apart(const Refs& grads) {
+  std::vector<Region> regions;
+  regions.reserve(grads.size());
+  for (const Tensor* g : grads) {
+    if (g->numel() == 0) continue;
+    regions.emplace_back(*g);
+    TORCH_CHECK_VALUE(!regions.back().own_overlap, "a gradient of shape ", g->sizes(), " and strides ", g->strides(),
+                      " shares memory between its own elements");
+  }
+  std::sort(regions.begin(), regions.end(), [](const Region& a, const Region& b) { return a.base < b.base; });
+  int64_t steps = int64_t{1} << 22;
+  for (size_t i = 0; i < regions.size(); ++i)
+    for (size_t j = i + 1; j < regions.size() && regions[j].base < regions[i].base + regions[i].span; ++j)
+      TORCH_CHECK_VALUE(!meet(regions[i], 0, regions[i].base, regions[j], 0, regions[j].base, &steps),
+                        "gradients overlap in memory (the same one listed twice?), or are too finely interleaved "
+                        "to tell");
+}
+
 // The kernels' call: norm of dense `src`, and with `dst` their scaled copies.
 Tensor clip(const Refs& src, const Refs* dst, float max_norm, int kind, const Tensor& norm_in) {
   const size_t n = src.size();
@@ -474,17 +545,9 @@ Tensor clip_in_place(const py::list& list, double max_norm, double norm_type, bo
   if (grads.empty()) return at::zeros({}, at::kFloat);
   check_list("grad", grads);
   Refs strided;
-  for (const Tensor* g : grads) {
-    if (g->is_contiguous()) continue;
-    for (int64_t d = 0; d < g->dim(); ++d)
-      TORCH_CHECK_VALUE(g->stride(d) != 0 || g->size(d) <= 1, "a gradient of shape ", g->sizes(),
-                        " shares memory between its own elements");
-    for (const Tensor* o : strided)
-      TORCH_CHECK_VALUE(!(o->const_data_ptr() == g->const_data_ptr() && o->sizes() == g->sizes() &&
-                          o->strides() == g->strides()),
-                        "gradients overlap in memory (the same one listed twice?)");
-    strided.push_back(g);
-  }
+  for (const Tensor* g : grads)
+    if (!g->is_contiguous()) strided.push_back(g);
+  if (!strided.empty()) check_apart(grads);
   std::vector<Tensor> copies;
   const Refs ts = dense(grads, &copies);
   Tensor norm_in;
