@@ -22,8 +22,11 @@ the streams. There is no CPU fallback: CPU tensors raise ``ValueError``.
 
 from __future__ import annotations
 
+import dis
 import functools
 import importlib
+import inspect
+import types
 from typing import Any, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -121,9 +124,102 @@ def _conditional_block_forward(block: torch.nn.Module, x: torch.Tensor, c: torch
     return x + gate_m * block.mlp(ada_layer_norm(_float32_under_autocast(x), shift_m, scale_m, block.norm2.eps))
 
 
+def _torch_norm(m: Any) -> bool:
+    """A LayerNorm over the last dim that computes what torch's does."""
+    return (isinstance(m, torch.nn.LayerNorm) and type(m).forward is torch.nn.LayerNorm.forward
+            and len(m.normalized_shape) == 1)
+
+
 def _plain_norm(m: Any) -> bool:
-    """A LayerNorm over the last dim without an affine."""
-    return isinstance(m, torch.nn.LayerNorm) and len(m.normalized_shape) == 1 and m.weight is None and m.bias is None
+    """A LayerNorm over the last dim without an affine, as torch computes it or routed here."""
+    own = getattr(m, "__dict__", {}).get("forward")
+    return (_torch_norm(m) and m.weight is None and m.bias is None
+            and (own is None or getattr(own, "func", None) is _layer_norm_forward))
+
+
+# What a block's forward computes is read by running it on stand-ins that write down what is done to them,
+# and compared with the formula that ``_conditional_block_forward`` computes.
+class _Value:
+    """How a value of a forward pass is made, as nested tuples; sums and products in one order."""
+
+    __slots__ = ("made",)
+
+    def __init__(self, *made: Any):
+        self.made = made
+
+    @staticmethod
+    def _of(v: Any) -> tuple:
+        if isinstance(v, _Value):
+            return v.made
+        if isinstance(v, (int, float)):
+            return ("number", float(v))
+        raise TypeError("not a value")
+
+    def __add__(self, other: Any) -> "_Value":
+        return _Value("+", *sorted((self.made, _Value._of(other)), key=repr))
+
+    def __mul__(self, other: Any) -> "_Value":
+        return _Value("*", *sorted((self.made, _Value._of(other)), key=repr))
+
+    __radd__, __rmul__ = __add__, __mul__
+
+    def chunk(self, chunks: int, dim: int = 0) -> tuple:
+        return tuple(_Value("chunk", self.made, chunks, dim, i) for i in range(chunks))
+
+
+class _Parts:
+    """A block whose parts write down that they were called; it has nothing else, and nothing can be set."""
+
+    __slots__ = ()
+
+    def __getattr__(self, name: str):
+        if name not in ("adaLN_modulation", "attn", "mlp", "norm1", "norm2"):
+            raise AttributeError(name)
+        return lambda v: _Value(name, _Value._of(v))
+
+
+def _conditional_block_formula(block, x, c):
+    """``ConditionalBlock.forward`` (reference ``lewm/module.py:105-111``)."""
+    shift_a, scale_a, gate_a, shift_m, scale_m, gate_m = block.adaLN_modulation(c).chunk(6, dim=-1)
+    x = x + gate_a * block.attn(block.norm1(x) * (1 + scale_a) + shift_a)
+    return x + gate_m * block.mlp(block.norm2(x) * (1 + scale_m) + shift_m)
+
+
+def _straight_line(f: Any, depth: int = 4) -> bool:
+    """Whether ``f`` is a Python function that takes one way through its code, whatever else there is: no
+    jumps, closures or handlers, nothing stored but its own variables, and of the globals only such functions."""
+    if not isinstance(f, types.FunctionType) or depth == 0:
+        return False
+    code = f.__code__
+    if code.co_freevars or code.co_cellvars or code.co_exceptiontable or f.__defaults__ or f.__kwdefaults__:
+        return False
+    for i in dis.get_instructions(code):
+        if i.opcode in dis.hasjrel or i.opcode in dis.hasjabs or i.opname.startswith(("IMPORT", "MAKE", "DELETE")):
+            return False
+        if i.opname.startswith("STORE_") and not i.opname.startswith("STORE_FAST"):
+            return False
+        if i.opname == "LOAD_GLOBAL" and not _straight_line(f.__globals__.get(i.argval), depth - 1):
+            return False
+    return True
+
+
+def _known_block(m: torch.nn.Module) -> bool:
+    """An AdaLN conditional block whose forward is the known formula."""
+    forward = type(m).forward
+    if (type(m).__name__ != "ConditionalBlock" or not all(hasattr(m, n) for n in ("adaLN_modulation", "attn", "mlp"))
+            or not _plain_norm(getattr(m, "norm1", None)) or not _plain_norm(getattr(m, "norm2", None))
+            or not _straight_line(forward)):
+        return False
+    code = forward.__code__
+    if code.co_argcount != 3 or code.co_kwonlyargcount or code.co_varnames[1:3] != ("x", "c") or \
+            code.co_flags & (inspect.CO_VARARGS | inspect.CO_VARKEYWORDS | inspect.CO_GENERATOR | inspect.CO_COROUTINE):
+        return False
+    x, c = _Value("x"), _Value("c")
+    try:
+        got = forward(_Parts(), x, c)
+    except Exception:  # it does something else than the formula needs
+        return False
+    return isinstance(got, _Value) and got.made == _conditional_block_formula(_Parts(), x, c).made
 
 
 class B200TrainingNorms:
@@ -135,11 +231,9 @@ class B200TrainingNorms:
         for name, m in model.named_modules():
             if "forward" in m.__dict__:  # routed already, by this or another install
                 continue
-            if type(m).forward is torch.nn.LayerNorm.forward and len(m.normalized_shape) == 1:
+            if _torch_norm(m):
                 m.forward = functools.partial(_layer_norm_forward, m)
-            elif (type(m).__name__ == "ConditionalBlock"
-                  and all(hasattr(m, n) for n in ("adaLN_modulation", "attn", "mlp"))
-                  and _plain_norm(getattr(m, "norm1", None)) and _plain_norm(getattr(m, "norm2", None))):
+            elif _known_block(m):
                 m.forward = functools.partial(_conditional_block_forward, m)
             else:
                 continue
@@ -155,7 +249,7 @@ class B200TrainingNorms:
 
 def install_training_norms(model: torch.nn.Module) -> B200TrainingNorms:
     """Route every ``nn.LayerNorm`` over the last dim (not subclasses with a forward of their own) and
-    every AdaLN ``ConditionalBlock`` of ``model`` (reference ``lewm/module.py:38-53,56-111,131-187,217-240``:
+    every AdaLN ``ConditionalBlock`` of ``model`` whose forward computes the known formula (reference ``lewm/module.py:38-53,56-111,131-187,217-240``:
     predictor, projector heads, and the ViT encoder) through ``layer_norm`` and ``ada_layer_norm``, so
     that a training step of the world model runs their forward and backward passes on the B200
     kernels. Parameters, state dict and
