@@ -117,11 +117,26 @@ def _layer_norm_forward(module: torch.nn.LayerNorm, x: torch.Tensor) -> torch.Te
     return layer_norm(_float32_under_autocast(x), module.weight, module.bias, module.eps)
 
 
+def _watched(m: torch.nn.Module) -> bool:
+    """Whether a hook wants to see the module called."""
+    return bool(m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks
+                or torch.nn.modules.module._has_any_global_hook())
+
+
+def _modulated_norm(norm: torch.nn.LayerNorm, x: torch.Tensor, shift: torch.Tensor,
+                    scale: torch.Tensor) -> torch.Tensor:
+    """``modulate(norm(x), shift, scale)``: in one pass where nothing else is asked of ``norm``, as a block's
+    norms may have been hooked or changed since they were routed."""
+    if _plain_norm(norm) and not _watched(norm):
+        return ada_layer_norm(_float32_under_autocast(x), shift, scale, norm.eps)
+    return norm(x) * (1 + scale) + shift
+
+
 def _conditional_block_forward(block: torch.nn.Module, x: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
     """``ConditionalBlock.forward`` (reference ``lewm/module.py:105-111``)."""
     shift_a, scale_a, gate_a, shift_m, scale_m, gate_m = block.adaLN_modulation(c).chunk(6, dim=-1)
-    x = x + gate_a * block.attn(ada_layer_norm(_float32_under_autocast(x), shift_a, scale_a, block.norm1.eps))
-    return x + gate_m * block.mlp(ada_layer_norm(_float32_under_autocast(x), shift_m, scale_m, block.norm2.eps))
+    x = x + gate_a * block.attn(_modulated_norm(block.norm1, x, shift_a, scale_a))
+    return x + gate_m * block.mlp(_modulated_norm(block.norm2, x, shift_m, scale_m))
 
 
 def _torch_norm(m: Any) -> bool:

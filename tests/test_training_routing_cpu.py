@@ -140,3 +140,116 @@ def test_blocks_with_norms_of_their_own_are_left_alone():
     block = block_class(reference_spelling)(8, 1, 8, 8)
     block.norm1.forward = lambda x: 3 * x
     assert lf.install_training_norms(block).modules == ["attn.norm", "mlp.0", "norm2"]
+
+
+# ---------------------------------------------------------------------------- routed blocks
+def plain_layer_norm(x, weight=None, bias=None, eps=1e-5):
+    return torch.nn.functional.layer_norm(x, x.shape[-1:], weight, bias, eps)
+
+
+def plain_ada_layer_norm(x, shift, scale, eps=1e-6):
+    """The kernel's contract: modulation of x's shape, or of size 1 in dims right before the last; x's type."""
+    m = (1,) * (x.dim() - shift.dim()) + tuple(shift.shape)
+    d = x.dim() - 2
+    while d >= 0 and m[d] == 1:
+        d -= 1
+    assert m == tuple(x.shape) or (m[-1] == x.shape[-1] and m[:d + 1] == tuple(x.shape)[:d + 1])
+    y = plain_layer_norm(x.double(), eps=eps) * (1 + scale.double()) + shift.double()
+    return y.to(x.dtype)
+
+
+@pytest.fixture
+def plain_forms(monkeypatch):
+    """The operators in plain torch, so that routed modules run on the CPU; counts their calls."""
+    calls = {"layer_norm": 0, "ada_layer_norm": 0}
+
+    def counting(name, f):
+        def g(*args, **kwargs):
+            calls[name] += 1
+            return f(*args, **kwargs)
+        return g
+
+    monkeypatch.setattr(training, "layer_norm", counting("layer_norm", plain_layer_norm))
+    monkeypatch.setattr(training, "ada_layer_norm", counting("ada_layer_norm", plain_ada_layer_norm))
+    return calls
+
+
+def a_block():
+    torch.manual_seed(0)
+    return training_reference.ConditionalBlock(16, 2, 8, 32)
+
+
+def close(a, b):
+    return torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+def test_block_calls_each_norm_once_in_one_pass(plain_forms):
+    block, x, c = a_block(), torch.randn(2, 3, 16), torch.randn(2, 3, 16)
+    want = block(x, c)
+    lf.install_training_norms(block)
+    assert close(block(x, c), want)
+    assert plain_forms == {"layer_norm": 2, "ada_layer_norm": 2}  # attn.norm and mlp.0
+
+
+@pytest.mark.parametrize("register", [
+    lambda n, f: n.register_forward_hook(lambda m, i, o: f(o)),
+    lambda n, f: n.register_forward_pre_hook(lambda m, i: f(i[0].sin())),  # a norm undoes a factor
+    lambda n, f: n.register_forward_hook(lambda m, i, k, o: f(o), with_kwargs=True),
+    lambda n, f: n.register_full_backward_hook(lambda m, gi, go: (f(gi[0]),)),
+    lambda n, f: n.register_full_backward_pre_hook(lambda m, go: (f(go[0]),)),
+], ids=["forward", "forward_pre", "forward_kwargs", "backward", "backward_pre"])
+@pytest.mark.parametrize("when", ["before", "after"])
+def test_hooks_on_a_blocks_norms_run(plain_forms, register, when):
+    """Hooks that double what they see, on both norms, set before or after routing."""
+    block, x, c = a_block(), torch.randn(2, 3, 16, requires_grad=True), torch.randn(2, 3, 16)
+    calls = []
+
+    def double(t):
+        calls.append(t.shape)
+        return 2 * t
+
+    def run():
+        return block(x, c), *torch.autograd.grad(block(x, c).square().sum(), x)
+
+    plain = run()
+    if when == "after":
+        handle = lf.install_training_norms(block)
+    hooks = [register(n, double) for n in (block.norm1, block.norm2)]
+    if when == "before":
+        handle = lf.install_training_norms(block)
+    got, seen = run(), len(calls)
+    handle.remove()
+    want = run()
+    assert len(calls) == 2 * seen and seen >= 2
+    assert all(close(p, q) for p, q in zip(got, want)) and not close(want[1], plain[1])
+    for h in hooks:
+        h.remove()
+
+
+def test_hooks_on_all_modules_see_a_blocks_norms(plain_forms):
+    block, x, c = a_block(), torch.randn(2, 3, 16), torch.randn(2, 3, 16)
+    lf.install_training_norms(block)
+    seen = []
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda m, i, o: seen.append(m))
+    try:
+        block(x, c)
+    finally:
+        hook.remove()
+    assert block.norm1 in seen and block.norm2 in seen
+
+
+def test_a_blocks_norms_may_change_after_routing(plain_forms):
+    block, x, c = a_block(), torch.randn(2, 3, 16), torch.randn(2, 3, 16)
+    handle = lf.install_training_norms(block)
+    block.norm1 = torch.nn.LayerNorm(16)  # with an affine
+    with torch.no_grad():
+        block.norm1.weight.mul_(3.0)
+    block.norm2.eps = 0.5
+    got = block(x, c)
+    handle.remove()
+    assert close(got, block(x, c))
+    block = a_block()
+    lf.install_training_norms(block)
+    block.norm2 = torch.nn.Identity()
+    got = block(x, c)
+    assert close(got, type(block).forward(block, x, c))
