@@ -123,12 +123,31 @@ def _watched(m: torch.nn.Module) -> bool:
                 or torch.nn.modules.module._has_any_global_hook())
 
 
+def _modulates(m: torch.Tensor, x: torch.Tensor) -> bool:
+    """Whether ``ada_layer_norm`` takes modulation ``m`` for ``x`` and gives what torch's products and sums
+    would: a row of ``m`` for each or for consecutive rows of ``x``, and no type above that of ``x``."""
+    if m.dtype != x.dtype and torch.promote_types(m.dtype, x.dtype) != x.dtype:
+        return False
+    ms, xs = m.shape, x.shape
+    if ms == xs:
+        return True
+    if not 0 < len(ms) <= len(xs) or ms[-1] != xs[-1]:
+        return False
+    ms = (1,) * (len(xs) - len(ms)) + tuple(ms)
+    d = len(ms) - 2
+    while d >= 0 and ms[d] == 1:
+        d -= 1
+    return ms[:d + 1] == tuple(xs[:d + 1])
+
+
 def _modulated_norm(norm: torch.nn.LayerNorm, x: torch.Tensor, shift: torch.Tensor,
                     scale: torch.Tensor) -> torch.Tensor:
-    """``modulate(norm(x), shift, scale)``: in one pass where nothing else is asked of ``norm``, as a block's
-    norms may have been hooked or changed since they were routed."""
+    """``modulate(norm(x), shift, scale)``: in one pass where the kernel has the form and nothing else is asked
+    of ``norm``, as a block's norms may have been hooked or changed since they were routed."""
     if _plain_norm(norm) and not _watched(norm):
-        return ada_layer_norm(_float32_under_autocast(x), shift, scale, norm.eps)
+        rows = _float32_under_autocast(x)
+        if _modulates(shift, rows):
+            return ada_layer_norm(rows, shift, scale, norm.eps)
     return norm(x) * (1 + scale) + shift
 
 

@@ -253,3 +253,52 @@ def test_a_blocks_norms_may_change_after_routing(plain_forms):
     block.norm2 = torch.nn.Identity()
     got = block(x, c)
     assert close(got, type(block).forward(block, x, c))
+
+
+@pytest.mark.parametrize("x,c", [
+    ((2, 3, 16), (3, 16)),        # one window's conditioning for all
+    ((2, 3, 16), (1, 3, 16)),
+    ((2, 3, 16), (16,)),
+    ((2, 3, 16), (2, 1, 16)),
+    ((2, 3, 16), (1, 1, 16)),
+    ((2, 1, 16), (2, 3, 16)),     # the result grows
+    ((1, 3, 16), (2, 3, 16)),
+    ((2, 1, 16), (2, 1, 16)),
+])
+def test_conditioning_of_any_shape_that_broadcasts(plain_forms, x, c):
+    block, x, c = a_block(), torch.randn(x), torch.randn(c)
+    want = block(x, c)
+    lf.install_training_norms(block)
+    got = block(x, c)
+    assert got.shape == want.shape and close(got, want)
+
+
+class Cast(torch.nn.Module):
+    """Keeps a block's parts in float32 behind a stream of another type."""
+
+    def __init__(self, inner, out=None):
+        super().__init__()
+        self.inner, self.out = inner, out
+
+    def forward(self, x):
+        y = self.inner(x.float())
+        return y if self.out is None else y.to(self.out)
+
+
+@pytest.mark.parametrize("stream", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mod", [torch.float32, torch.bfloat16, torch.float16])
+def test_types_promote_as_they_did(plain_forms, stream, mod):
+    """A modulation type above that of x lifts the result, as in torch: float32 stays float32 behind bf16 rows."""
+    block = a_block()
+    seen = []
+    block.attn, block.mlp = Cast(block.attn), Cast(block.mlp)
+    block.adaLN_modulation = Cast(block.adaLN_modulation, mod)
+    for m in (block.attn, block.mlp):
+        m.register_forward_pre_hook(lambda m, i: seen.append(i[0].dtype))
+    x, c = torch.randn(2, 3, 16).to(stream), torch.randn(2, 3, 16)
+    want = block(x, c)
+    lf.install_training_norms(block)
+    got = block(x, c)
+    assert got.dtype == want.dtype and seen[:2] == seen[2:]
+    assert torch.allclose(got.float(), want.float(), rtol=0.05, atol=0.05)  # a few roundings to 2^-8 of values of 4
+    assert seen[0] == torch.promote_types(stream, mod)
