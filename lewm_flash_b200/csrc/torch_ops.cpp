@@ -72,7 +72,24 @@ void check_no_tangent(const char* name, const Tensor& t) {
                               "forward-mode derivative");
 }
 
+// Tensors that stand for others, with no memory of their own or not theirs alone to interpret: what
+// torch.func's transforms (vmap, grad, functionalize) and batched gradients pass in, and subclasses with a
+// __torch_dispatch__ (DTensor, FakeTensor).
+bool is_wrapper(const Tensor& t) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet keys({DispatchKey::FuncTorchBatched, DispatchKey::BatchedNestedTensor,
+                                      DispatchKey::Batched, DispatchKey::FuncTorchGradWrapper,
+                                      DispatchKey::Functionalize, DispatchKey::Python, DispatchKey::ZeroTensor});
+  return t.key_set().has_any(keys);
+}
+
+void check_no_wrapper(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!is_wrapper(t), name, " belongs to a transform (torch.func, vmap, batched gradients) or "
+                              "is a subclass with a __torch_dispatch__: the B200 training operators take plain tensors");
+}
+
 void check_tensor(const char* name, const Tensor& t) {
+  check_no_wrapper(name, t);
   TORCH_CHECK_VALUE(type_code(t) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
   TORCH_CHECK_VALUE(t.layout() == at::kStrided, name, " must be a dense tensor, got layout ", t.layout());
   TORCH_CHECK_VALUE(!t.is_neg(), name, " is a lazily negated view: pass it through resolve_neg()");
@@ -181,6 +198,7 @@ struct NormBackward : public torch::autograd::Node {
                need_b = has_b && task_should_compute_output(2);
     if (!dy.defined() || !(need_x || need_a || need_b)) return out;
     check_no_tracer();
+    check_no_wrapper("the output's gradient", dy);
     check_no_tangent("the output's gradient", dy);
     Tensor x, a, stats;
     {
@@ -341,7 +359,7 @@ Refs refs(const char* name, const py::list& list) {
 void check_list(const char* name, const Refs& ts) {
   for (size_t i = 0; i < ts.size(); ++i) {
     const Tensor& t = *ts[i];
-    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg() || has_tangent(t))
+    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg() || is_wrapper(t) || has_tangent(t))
       check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
     TORCH_CHECK_VALUE(t.device() == ts[0]->device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
                       ts[0]->device(), ": one device per call");
@@ -527,7 +545,7 @@ std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, do
                           o.device() == g.device(),
                       "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
     TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");
-    if (has_tangent(o)) check_no_tangent(("out[" + std::to_string(i) + "]").c_str(), o);
+    if (is_wrapper(o) || has_tangent(o)) check_tensor(("out[" + std::to_string(i) + "]").c_str(), o);
   }
   std::vector<Tensor> copies;
   Tensor norm = clip(dense(grads, &copies), &out, limit, kind, Tensor());

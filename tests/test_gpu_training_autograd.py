@@ -136,3 +136,11 @@ def test_lazily_negated_output_gradient(rows, width):
     want = torch.autograd.grad(y, (x, shift, scale), -dy, retain_graph=True)
     got = torch.autograd.grad(y, (x, shift, scale), torch._neg_view(dy))
     assert all(torch.equal(p, q) and not p.is_neg() for p, q in zip(got, want))
+
+
+# ---------------------------------------------------------------------------- function transforms, subclasses
+def test_batched_output_gradients_are_refused():
+    x = randn(4, 32).requires_grad_(True)
+    y = lf.layer_norm(x)
+    with pytest.raises(NotImplementedError, match="torch.func"):
+        torch.autograd.grad(y, x, randn(3, 4, 32, seed=1), is_grads_batched=True)

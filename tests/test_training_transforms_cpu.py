@@ -59,3 +59,51 @@ def test_tracing_is_refused(call, trace):
         trace(call, z(3, 8))
     with pytest.raises(ValueError, match="need a CUDA device"):
         call(z(3, 8))
+
+
+# ---------------------------------------------------------------------------- function transforms, subclasses
+TRANSFORMS = {
+    "vmap": lambda f: torch.vmap(f)(z(2, 3, 8)),
+    "grad": lambda f: torch.func.grad(lambda t: f(t).sum())(z(3, 8)),
+    "jvp": lambda f: torch.func.jvp(f, (z(3, 8),), (z(3, 8),)),
+    "jacrev": lambda f: torch.func.jacrev(f)(z(3, 8)),
+    "jacfwd": lambda f: torch.func.jacfwd(f)(z(3, 8)),
+    "functionalize": lambda f: torch.func.functionalize(f)(z(3, 8)),
+}
+CALLS = [lambda x: lf.layer_norm(x), lambda x: lf.layer_norm(z(3, 8), x[0]), lambda x: lf.ada_layer_norm(x, z(8), z(8)),
+         lambda x: lf.ada_layer_norm(z(3, 8), z(3, 8), x), lambda x: lf.grad_norm([z(2), x]),
+         lambda x: lf.clip_grads([x], 1.0)[1], lambda x: lf.clip_grads([z(8)], 1.0, out=[x[0]])[1]]
+
+
+@pytest.mark.parametrize("transform", list(TRANSFORMS.values()), ids=list(TRANSFORMS))
+@pytest.mark.parametrize("call", CALLS)
+def test_function_transforms_are_refused_by_name(call, transform):
+    with pytest.raises(NotImplementedError, match="torch.func"):
+        transform(call)
+
+
+def test_function_transforms_around_plain_tensors_are_fine():
+    plain = z(3, 8)
+
+    def f(x):
+        lf.layer_norm(plain)
+        return x
+
+    for transform in TRANSFORMS.values():
+        with pytest.raises(ValueError, match="need a CUDA device"):
+            transform(f)
+
+
+def test_dispatching_subclasses_are_refused_by_name():
+    class Wrapped(torch.Tensor):
+        __torch_function__ = torch._C._disabled_torch_function_impl
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return NotImplemented
+
+    x = torch.Tensor._make_subclass(Wrapped, z(3, 8))
+    with pytest.raises(NotImplementedError, match="__torch_dispatch__"):
+        lf.layer_norm(x)
+    with pytest.raises(NotImplementedError, match="__torch_dispatch__"):
+        lf.clip_grads([z(3), x], 1.0)
