@@ -30,6 +30,7 @@ import types
 from typing import Any, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 
@@ -62,6 +63,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     the shape and type of ``x`` and is contiguous. ``x`` may be strided: rows that step evenly
     through memory are read in place, others are copied first. Differentiable once in all three.
     """
+    if has_torch_function_variadic(x, weight, bias):  # subclasses and modes see the call
+        return handle_torch_function(layer_norm, (x, weight, bias), x, weight, bias, eps)
     return _ops().layer_norm(x, weight, bias, eps)
 
 
@@ -74,6 +77,8 @@ def ada_layer_norm(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, ep
     left out. Chunks of an AdaLN Linear's output are read in place. The result has the shape and
     type of ``x`` and is contiguous; differentiable once in all three.
     """
+    if has_torch_function_variadic(x, shift, scale):
+        return handle_torch_function(ada_layer_norm, (x, shift, scale), x, shift, scale, eps)
     return _ops().ada_layer_norm(x, shift, scale, eps)
 
 

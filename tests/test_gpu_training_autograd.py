@@ -144,3 +144,15 @@ def test_batched_output_gradients_are_refused():
     y = lf.layer_norm(x)
     with pytest.raises(NotImplementedError, match="torch.func"):
         torch.autograd.grad(y, x, randn(3, 4, 32, seed=1), is_grads_batched=True)
+
+
+def test_tensor_subclasses_stay():
+    class Named(torch.Tensor):
+        pass
+
+    x, w = activation(20, 192, F32), randn(192, seed=2)
+    y = lf.layer_norm(x.as_subclass(Named), w)
+    assert type(y) is Named and torch.equal(y.as_subclass(torch.Tensor), lf.layer_norm(x, w))
+    y = lf.ada_layer_norm(x, w.as_subclass(Named), w)
+    assert type(y) is Named and torch.equal(y.as_subclass(torch.Tensor), lf.ada_layer_norm(x, w, w))
+    assert type(lf.layer_norm(torch.nn.Parameter(x), w)) is torch.Tensor

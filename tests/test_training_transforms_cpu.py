@@ -107,3 +107,27 @@ def test_dispatching_subclasses_are_refused_by_name():
         lf.layer_norm(x)
     with pytest.raises(NotImplementedError, match="__torch_dispatch__"):
         lf.clip_grads([z(3), x], 1.0)
+
+
+def test_subclasses_and_modes_see_the_norms():
+    class Recorder(torch.Tensor):
+        seen = []
+
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            cls.seen.append(func)
+            return "answered"
+
+    r = z(3, 8).as_subclass(Recorder)
+    assert lf.layer_norm(r) == "answered" and lf.layer_norm(z(3, 8), r) == "answered"
+    assert lf.ada_layer_norm(z(3, 8), z(8), r) == "answered"
+    assert Recorder.seen == [lf.layer_norm, lf.layer_norm, lf.ada_layer_norm]
+
+    class Mode(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func if func in (lf.layer_norm, lf.ada_layer_norm) else func(*args, **(kwargs or {}))
+
+    with Mode():
+        assert lf.layer_norm(z(3, 8)) is lf.layer_norm
+    with torch.device("cpu"), pytest.raises(ValueError, match="need a CUDA device"):
+        lf.layer_norm(z(3, 8))
