@@ -119,6 +119,8 @@ def _float32_under_autocast(x: torch.Tensor) -> torch.Tensor:
 
 
 def _layer_norm_forward(module: torch.nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    if x.dim() == 0 or x.shape[-1] != module.normalized_shape[0]:  # nothing else tells without weight and bias
+        raise ValueError(f"x of shape {tuple(x.shape)} does not end in the norm's {module.normalized_shape[0]}")
     return layer_norm(_float32_under_autocast(x), module.weight, module.bias, module.eps)
 
 
@@ -151,7 +153,7 @@ def _modulated_norm(norm: torch.nn.LayerNorm, x: torch.Tensor, shift: torch.Tens
     of ``norm``, as a block's norms may have been hooked or changed since they were routed."""
     if _plain_norm(norm) and not _watched(norm):
         rows = _float32_under_autocast(x)
-        if _modulates(shift, rows):
+        if _modulates(shift, rows) and x.shape[-1] == norm.normalized_shape[0]:
             return ada_layer_norm(rows, shift, scale, norm.eps)
     return norm(x) * (1 + scale) + shift
 

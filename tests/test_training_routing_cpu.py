@@ -302,3 +302,26 @@ def test_types_promote_as_they_did(plain_forms, stream, mod):
     assert got.dtype == want.dtype and seen[:2] == seen[2:]
     assert torch.allclose(got.float(), want.float(), rtol=0.05, atol=0.05)  # a few roundings to 2^-8 of values of 4
     assert seen[0] == torch.promote_types(stream, mod)
+
+
+# ---------------------------------------------------------------------------- what torch's modules refuse
+@pytest.mark.parametrize("affine", [False, True])
+@pytest.mark.parametrize("shape", [(3, 7), (3, 16, 1), ()])
+def test_rows_of_another_width_stay_refused(plain_forms, affine, shape):
+    norm = torch.nn.LayerNorm(16, elementwise_affine=affine)
+    with pytest.raises(RuntimeError):
+        norm(torch.zeros(shape))
+    lf.install_training_norms(norm)
+    with pytest.raises(ValueError, match="does not end in the norm's 16"):
+        norm(torch.zeros(shape))
+
+
+def test_blocks_of_another_width_stay_refused(plain_forms):
+    block = a_block()
+    block.norm1 = torch.nn.LayerNorm(8, elementwise_affine=False)
+    x, c = torch.randn(2, 3, 16), torch.randn(2, 3, 16)
+    with pytest.raises(RuntimeError):
+        block(x, c)
+    lf.install_training_norms(block)
+    with pytest.raises(ValueError, match="does not end in the norm's 8"):
+        block(x, c)
