@@ -114,8 +114,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
 
 # ---------------------------------------------------------------------------- a torch world model
 def _float32_under_autocast(x: torch.Tensor) -> torch.Tensor:
-    """torch runs layer_norm in float32 under autocast."""
-    return x.float() if torch.is_autocast_enabled("cuda") and x.is_floating_point() else x
+    """torch runs layer_norm in float32 under autocast; float64 stays (and is refused)."""
+    return x.float() if x.dtype in (torch.bfloat16, torch.float16) and torch.is_autocast_enabled("cuda") else x
 
 
 def _layer_norm_forward(module: torch.nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:

@@ -325,3 +325,16 @@ def test_blocks_of_another_width_stay_refused(plain_forms):
     lf.install_training_norms(block)
     with pytest.raises(ValueError, match="does not end in the norm's 8"):
         block(x, c)
+
+
+def test_float64_is_not_rounded_under_autocast(monkeypatch):
+    """torch keeps float64 there; the kernels have no float64."""
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device=None: True)
+    norm, block = torch.nn.LayerNorm(8), a_block().double()
+    lf.install_training_norms(norm), lf.install_training_norms(block)
+    with pytest.raises(ValueError, match="must be float32"):
+        norm(torch.zeros(3, 8, dtype=torch.float64))
+    with pytest.raises(ValueError, match="must be float32"):
+        block(*torch.zeros(2, 2, 3, 16, dtype=torch.float64))
+    with pytest.raises(ValueError, match="need a CUDA device"):
+        norm(torch.zeros(3, 8, dtype=torch.bfloat16))
