@@ -283,7 +283,8 @@ class B200TrainingNorms:
 
     def remove(self) -> None:
         for m in self._routed:
-            m.__dict__.pop("forward", None)
+            if getattr(m.__dict__.get("forward"), "func", None) in (_layer_norm_forward, _conditional_block_forward):
+                del m.__dict__["forward"]  # one set since then stays
         self._routed = []
         self.modules = []
 

@@ -338,3 +338,11 @@ def test_float64_is_not_rounded_under_autocast(monkeypatch):
         block(*torch.zeros(2, 2, 3, 16, dtype=torch.float64))
     with pytest.raises(ValueError, match="need a CUDA device"):
         norm(torch.zeros(3, 8, dtype=torch.bfloat16))
+
+
+def test_removal_leaves_forwards_set_since():
+    model = torch.nn.Sequential(torch.nn.LayerNorm(8), torch.nn.LayerNorm(8))
+    handle = lf.install_training_norms(model)
+    own = model[0].forward = lambda x: 3 * x
+    handle.remove()
+    assert model[0].__dict__["forward"] is own and "forward" not in model[1].__dict__
