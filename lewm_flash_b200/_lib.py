@@ -127,7 +127,6 @@ SIGNATURES = {
     "lewm_grad_clip": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_float,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
 }
-GRAD_WORKSPACE = 32768  # LEWM_GRAD_WORKSPACE
 KERNEL_CLASSES = ("embed", "adaln", "qkv_attn", "out_proj", "fc1", "fc2", "final", "sample", "refit", "prep0", "ffn",
                   "ln_operand", "tile_call", "fp32_cost")
 

@@ -259,3 +259,11 @@ def test_cem_gd_gradient_clip_must_be_positive(value):
     with pytest.raises(ValueError, match="gd_max_grad_norm must be positive"):
         lf.B200CEMGDSolver(model=None, gd_max_grad_norm=value)
     assert lf.B200CEMGDSolver(model=None).gd_max_grad_norm is None
+
+
+def test_header_sizes_have_no_second_copy():
+    """LEWM_GRAD_WORKSPACE stands in the header alone, where the extension takes it from: a copy in the
+    binding would go stale unnoticed, as lewm_grad_* cannot check what it is given."""
+    header = _lib.PKG.parent / "include" / "lewm_b200.h"
+    assert "#define LEWM_GRAD_WORKSPACE 32768" in header.read_text()
+    assert not [n for n in vars(_lib) if "WORKSPACE" in n]
