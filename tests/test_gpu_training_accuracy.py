@@ -86,3 +86,22 @@ def test_squares_that_overflow_stay_finite():
     assert torch.equal(lf.layer_norm(x[3:4], w, b), b.expand(1, -1))
     wide = randn(3, 20000, seed=4, scale=1e30)
     assert not lf.layer_norm(wide).any()
+
+
+# ---------------------------------------------------------------------------- every pairing of types
+@pytest.mark.parametrize("dtype,ctype", [(F32, BF16), (F32, F16), (BF16, F16), (F16, BF16), (BF16, BF16), (F16, F32)],
+                         ids=["f32-bf16", "f32-f16", "bf16-f16", "f16-bf16", "bf16", "f16-f32"])
+@pytest.mark.parametrize("batch,tokens,width", [(1, 1, 192), (300, 3, 192), (2000, 3, 192), (1700, 3, 384), (7, 5, 33),
+                                                (1000, 5, 70), (40, 15, 2050), (9, 40, 640), (5000, 1, 154),
+                                                (7, 30, 4100), (20, 3, 8192), (9, 4, 10008), (3, 2, 16385)])
+@pytest.mark.parametrize("shared", [False, True], ids=["per_token", "per_sequence"])
+def test_ada_layer_norm_of_mixed_types(batch, tokens, width, shared, dtype, ctype):
+    """float32 rows with 16-bit modulation are what a float32 model gives under autocast."""
+    x = activation(batch * tokens, width, dtype).view(batch, tokens, width).requires_grad_(True)
+    mod = randn(batch, 1 if shared else tokens, 6 * width, seed=3, scale=0.4, dtype=ctype)
+    shift, scale = (t.requires_grad_(True) for t in mod.chunk(6, -1)[:2])
+    dy = randn(batch, tokens, width, seed=7, scale=0.1, dtype=dtype)
+    y = lf.ada_layer_norm(x, shift, scale)
+    dx, dshift, dscale = torch.autograd.grad(y, (x, shift, scale), dy)
+    assert y.dtype == dtype and dshift.dtype == dscale.dtype == ctype
+    check_norm(x, scale, shift, 1e-6, True, tokens if shared else 1, y.detach(), dy, dx, dscale, dshift)
