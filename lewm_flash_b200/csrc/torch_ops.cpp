@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -62,10 +63,15 @@ void check_no_tracer() {
                               "(install_training_norms(...).remove())");
 }
 
-// A tangent (torch.autograd.forward_ad) that the kernels would drop.
-bool has_tangent(const Tensor& t) {
-  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::isFwGradDefined(t);
+// Whether tensors can have tangents at all: a level of torch.autograd.forward_ad is open. Asked once per
+// call; a look at each of 1046 tensors took a clip of 523 from 52 to 115 us.
+bool forward_mode() {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+         torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
 }
+
+// A tangent, which the kernels would drop.
+bool has_tangent(const Tensor& t) { return forward_mode() && t._fw_grad(0).defined(); }
 
 void check_no_tangent(const char* name, const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " has a tangent: the B200 training operators have no "
@@ -357,9 +363,10 @@ Refs refs(const char* name, const py::list& list) {
 }
 
 void check_list(const char* name, const Refs& ts) {
+  const bool tangents = forward_mode();
   for (size_t i = 0; i < ts.size(); ++i) {
     const Tensor& t = *ts[i];
-    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg() || is_wrapper(t) || has_tangent(t))
+    if (type_code(t) < 0 || t.layout() != at::kStrided || t.is_neg() || is_wrapper(t) || (tangents && has_tangent(t)))
       check_tensor((std::string(name) + "[" + std::to_string(i) + "]").c_str(), t);
     TORCH_CHECK_VALUE(t.device() == ts[0]->device(), name, "[", i, "] is on ", t.device(), ", ", name, "[0] on ",
                       ts[0]->device(), ": one device per call");
@@ -539,13 +546,14 @@ std::pair<py::list, Tensor> clip_grads(const py::list& list, double max_norm, do
     for (const Tensor* g : grads) out_list.append(empty(g->sizes(), g->scalar_type(), *g));
   }
   const Refs out = refs("out", out_list);
+  const bool tangents = forward_mode();
   for (size_t i = 0; out_given && i < grads.size(); ++i) {
     const Tensor &g = *grads[i], &o = *out[i];
     TORCH_CHECK_VALUE(o.layout() == at::kStrided && !o.is_neg() && o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() &&
                           o.device() == g.device(),
                       "out[", i, "] must be a ", g.scalar_type(), " tensor of shape ", g.sizes(), " on ", g.device());
     TORCH_CHECK_VALUE(o.is_contiguous(), "out[", i, "] must be contiguous");
-    if (is_wrapper(o) || has_tangent(o)) check_tensor(("out[" + std::to_string(i) + "]").c_str(), o);
+    if (is_wrapper(o) || (tangents && has_tangent(o))) check_tensor(("out[" + std::to_string(i) + "]").c_str(), o);
   }
   std::vector<Tensor> copies;
   Tensor norm = clip(dense(grads, &copies), &out, limit, kind, Tensor());
