@@ -392,7 +392,7 @@ typedef struct lewm_norm_desc {
 /* y = z a + b (layer norm) or z (1 + a) + b (adaptive), z = (x - mean) / sqrt(var + eps) with
  * the biased variance of the row; y [rows][width] contiguous. stats (float32 [2][rows]: mean,
  * then 1 / sqrt(var + eps)) is what the backward pass needs, or NULL. float32 arithmetic, one
- * rounding at the store. */
+ * rounding at the store; z of a constant row is 0 (widths to 2^15, eps > 0). */
 LEWM_API lewm_status lewm_norm_forward(const lewm_norm_desc* desc, const void* x, const void* a, const void* b,
                                        void* y, float* stats, int32_t device, void* stream);
 
@@ -409,7 +409,7 @@ LEWM_API lewm_status lewm_norm_backward(const lewm_norm_desc* desc, const void* 
                                         void* workspace, size_t workspace_bytes, int32_t device, void* stream);
 
 /* Kinds of gradient norm. */
-#define LEWM_NORM_L2 0  /* sqrt of the sum of squares, accumulated in float64 */
+#define LEWM_NORM_L2 0  /* sqrt of the sum of squares: float32 within 16 bytes, float64 beyond */
 #define LEWM_NORM_MAX 1 /* largest magnitude */
 
 /* Bytes of workspace of lewm_grad_norm and lewm_grad_clip. */

@@ -12,9 +12,9 @@
 //
 // Bound: bytes, 4 to 12 per element and pass. Many rows run at 91 to 102% of the rate of a plain copy
 // (131072 x 2048 bf16: forward 168 us, backward 261; 73881 x 1536 float32, groups of 8209 rows: 140 and
-// 206), at odd addresses at about 60%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
-// 35 and 51 us). A row therefore stays in registers from its only load to its only
-// store (mean and variance are two passes over registers), and sums over rows are kept in
+// 206), at odd addresses at about 55%: there a row costs 1.5 times the instructions (16384 x 2047 bf16:
+// 36 and 51 us). A row therefore stays in registers from its only load to its only
+// store (mean and variance are two passes over registers, row_stats), and sums over rows are kept in
 // registers by persistent blocks that own fixed columns, so x and dy are read once.
 //
 // Layout: a team of TPR threads holds one row, NV vectors of E elements per thread (vectors of 16, 8
@@ -27,8 +27,8 @@
 // three rows ahead: registers alone kept 32 KB per SM on the way at best and none while a row
 // was being reduced, half of HBM's rate (131072 x 2048 bf16: forward 307 us, backward 404).
 // With vectors each thread copies just what it reads itself, so the ring needs no barrier; rows
-// of odd 16-bit addresses (and odd float32 widths) are copied by 16-byte pieces with 4-byte ends and
-// read back element by element after a team barrier.
+// of odd 16-bit addresses (odd float32 widths, and rows off 16 bytes with a modulation row each) are copied
+// by 16-byte pieces with 4-byte ends and read back element by element after a team barrier.
 //
 // Work is cut into items: a run of rows within one group. An item is a block's (its teams
 // interleave the rows and add up through shared memory), or a team's where there are many
@@ -935,8 +935,8 @@ __global__ void __launch_bounds__(Tm::THREADS, kBound<Tm, ROW_BWD>) k_rowmod_bwd
 
 // ------------------------------------------------------------------ rows too wide for a block (is_wide)
 // A block per row, the row re-read (from L2) for each pass, in vectors of E elements.
-// Threads of a block, 2048 on an SM: 256, 512 and 1024 took 35, 33 and 39 us forward (1000 x 20000 bf16) and
-// 414, 424 and 530 us backward (16384 x 10000 bf16).
+// Threads of a block, 2048 on an SM: 256, 512 and 1024 took 35, 33 and 39 us forward (1000 x 20000 bf16; the
+// mean's second step adds 2 to each) and 414, 424 and 530 us backward (16384 x 10000 bf16).
 constexpr int kWideThreads = 512;
 using Wide = Team<1, 2, kWideThreads, 0>;
 

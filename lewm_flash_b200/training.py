@@ -13,11 +13,16 @@ memory-bound operators of that step around its matrix products:
   model (a reference ``JEPA``) through the first two, forward and backward.
 
 Tensors are float32, bfloat16 or float16 CUDA tensors; arithmetic, statistics and sums are float32
-(the norm's sum float64) and every result is rounded once. Calls run on the current stream of
-their tensors' device, allocate from torch's caching allocator, never synchronize (except
-``error_if_nonfinite``) and can be captured into CUDA graphs. Results do not depend on the run:
-no atomics. As with torch's own operators, a caller that hands tensors to another stream orders
-the streams. There is no CPU fallback: CPU tensors raise ``ValueError``.
+(the gradient norm's sum is float64 over sums of 4 or 8 squares in float32) and every result is rounded
+once. Calls run on the current stream of their tensors' device, allocate from torch's caching allocator,
+never synchronize (except ``error_if_nonfinite``) and can be captured into CUDA graphs. Results do not
+depend on the run: no atomics. As with torch's own operators, a caller that hands tensors to another
+stream orders the streams. There is no CPU fallback: CPU tensors raise ``ValueError``.
+
+The norms are differentiable once, in reverse. What would need more raises ``NotImplementedError``
+instead of going wrong: forward-mode derivatives, tracers (``torch.jit.trace``, ``make_fx``,
+``torch.export``), the transforms of ``torch.func`` and subclasses with a ``__torch_dispatch__``. Other
+subclasses and modes see the norms through ``__torch_function__``.
 """
 
 from __future__ import annotations
@@ -104,8 +109,9 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     """``torch.nn.utils.clip_grad_norm_`` on the kernels: scales the ``grad`` of every parameter in
     place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm (0-d float32).
 
-    The gradients are on one CUDA device and do not overlap. ``error_if_nonfinite`` reads the norm
-    on the host (so not under graph capture) and raises before anything is scaled."""
+    The gradients are on one CUDA device and do not overlap: those that share memory, strided ones
+    included, are refused (strided views that only interleave are not). ``error_if_nonfinite`` reads the
+    norm on the host (so not under graph capture) and raises before anything is scaled."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [g for g in (p.grad for p in parameters) if g is not None]
@@ -291,10 +297,12 @@ class B200TrainingNorms:
 
 def install_training_norms(model: torch.nn.Module) -> B200TrainingNorms:
     """Route every ``nn.LayerNorm`` over the last dim (not subclasses with a forward of their own) and
-    every AdaLN ``ConditionalBlock`` of ``model`` whose forward computes the known formula (reference ``lewm/module.py:38-53,56-111,131-187,217-240``:
-    predictor, projector heads, and the ViT encoder) through ``layer_norm`` and ``ada_layer_norm``, so
-    that a training step of the world model runs their forward and backward passes on the B200
-    kernels. Parameters, state dict and
-    autocast behaviour stay as they are: under autocast the norms run in float32 as torch's do.
-    The model's inputs must be on a CUDA device."""
+    every AdaLN ``ConditionalBlock`` of ``model`` whose forward computes the known formula (reference
+    ``lewm/module.py:38-53,56-111,131-187,217-240``: predictor, projector heads, and the ViT encoder)
+    through ``layer_norm`` and ``ada_layer_norm``, so that a training step of the world model runs their
+    forward and backward passes on the B200 kernels. Parameters, state dict, hooks, type promotion and autocast behaviour stay as they are: under
+    autocast the norms run in float32 as torch's do, and a block whose norms are hooked or were changed, or
+    whose modulation broadcasts in a way the kernel has not, calls the norm and modulates by itself.
+    The model's inputs must be on a CUDA device and not float64. Remove the routing to trace or export the
+    model, or to take forward-mode derivatives."""
     return B200TrainingNorms(model)
