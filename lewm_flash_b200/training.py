@@ -252,11 +252,11 @@ def _straight_line(f: Any, depth: int = 4) -> bool:
 
 def _known_block(m: torch.nn.Module) -> bool:
     """An AdaLN conditional block whose forward is the known formula."""
-    forward = type(m).forward
     if (type(m).__name__ != "ConditionalBlock" or not all(hasattr(m, n) for n in ("adaLN_modulation", "attn", "mlp"))
             or not _plain_norm(getattr(m, "norm1", None)) or not _plain_norm(getattr(m, "norm2", None))
-            or not _straight_line(forward)):
+            or not _straight_line(type(m).forward)):
         return False
+    forward = type(m).forward
     code = forward.__code__
     if code.co_argcount != 3 or code.co_kwonlyargcount or code.co_varnames[1:3] != ("x", "c") or \
             code.co_flags & (inspect.CO_VARARGS | inspect.CO_VARKEYWORDS | inspect.CO_GENERATOR | inspect.CO_COROUTINE):

@@ -346,3 +346,15 @@ def test_removal_leaves_forwards_set_since():
     own = model[0].forward = lambda x: 3 * x
     handle.remove()
     assert model[0].__dict__["forward"] is own and "forward" not in model[1].__dict__
+
+
+class Doubled(torch.nn.Module):
+    def forward(self, x):
+        return 2 * x
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_models_with_scripted_parts_are_routed_around_them():
+    model = torch.nn.Sequential(torch.jit.script(Doubled()), torch.jit.trace(Doubled(), torch.zeros(2)),
+                                torch.jit.script(torch.nn.LayerNorm(8)), torch.nn.LayerNorm(8))
+    assert lf.install_training_norms(model).modules == ["3"]
