@@ -124,10 +124,10 @@ def _float32_under_autocast(x: torch.Tensor) -> torch.Tensor:
     return x.float() if x.dtype in (torch.bfloat16, torch.float16) and torch.is_autocast_enabled("cuda") else x
 
 
-def _layer_norm_forward(module: torch.nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
-    if x.dim() == 0 or x.shape[-1] != module.normalized_shape[0]:  # nothing else tells without weight and bias
-        raise ValueError(f"x of shape {tuple(x.shape)} does not end in the norm's {module.normalized_shape[0]}")
-    return layer_norm(_float32_under_autocast(x), module.weight, module.bias, module.eps)
+def _layer_norm_forward(module: torch.nn.LayerNorm, input: torch.Tensor) -> torch.Tensor:
+    if input.dim() == 0 or input.shape[-1] != module.normalized_shape[0]:  # nothing else tells without weight and bias
+        raise ValueError(f"input of shape {tuple(input.shape)} does not end in the norm's {module.normalized_shape[0]}")
+    return layer_norm(_float32_under_autocast(input), module.weight, module.bias, module.eps)
 
 
 def _watched(m: torch.nn.Module) -> bool:

@@ -358,3 +358,11 @@ def test_models_with_scripted_parts_are_routed_around_them():
     model = torch.nn.Sequential(torch.jit.script(Doubled()), torch.jit.trace(Doubled(), torch.zeros(2)),
                                 torch.jit.script(torch.nn.LayerNorm(8)), torch.nn.LayerNorm(8))
     assert lf.install_training_norms(model).modules == ["3"]
+
+
+def test_routed_modules_take_their_arguments_by_name(plain_forms):
+    norm, block = torch.nn.LayerNorm(16), a_block()
+    x, c = torch.randn(2, 3, 16), torch.randn(2, 3, 16)
+    want = norm(input=x), block(x, c=c), block(c=c, x=x)
+    lf.install_training_norms(norm), lf.install_training_norms(block)
+    assert all(close(p, q) for p, q in zip((norm(input=x), block(x, c=c), block(c=c, x=x)), want))
