@@ -156,3 +156,36 @@ def test_tensor_subclasses_stay():
     y = lf.ada_layer_norm(x, w.as_subclass(Named), w)
     assert type(y) is Named and torch.equal(y.as_subclass(torch.Tensor), lf.ada_layer_norm(x, w, w))
     assert type(lf.layer_norm(torch.nn.Parameter(x), w)) is torch.Tensor
+
+
+# ---------------------------------------------------------------------------- a routed model
+def test_routed_model_saved_loaded_and_run_under_autograds_modes():
+    import io
+
+    from tests.training_reference import TinyPredictor
+
+    torch.manual_seed(0)
+    model = TinyPredictor().to(DEV)
+    lf.install_training_norms(model)
+    x, c = randn(5, 3, 64, seed=1).requires_grad_(True), randn(5, 3, 64, seed=2)
+
+    def grad():
+        (g,) = torch.autograd.grad(model(x, c).square().sum(), x)
+        return g
+
+    want = grad()
+    with torch.autograd.set_detect_anomaly(True):
+        assert torch.equal(grad(), want)
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or t.clone(), lambda t: t):
+        y = model(x, c)
+    assert torch.equal(torch.autograd.grad(y.square().sum(), x)[0], want) and packed
+    buf = io.BytesIO()
+    torch.save(model, buf)
+    buf.seek(0)
+    loaded = torch.load(buf, weights_only=False)
+    assert torch.equal(loaded(x, c), model(x, c))
+    with torch.no_grad():
+        for p in loaded.parameters():
+            p.zero_()
+    assert not loaded(x, c).any() and model(x, c).any()  # its own parameters
